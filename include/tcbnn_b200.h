@@ -391,6 +391,48 @@ int tcbnn_mma_operand_probe(int n, int a_off16, int iters, double* clocks_per_mm
 int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, double* issue_clocks_per_copy,
                          double* bytes_per_clock);
 
+/* ---- products of real-valued rows, and scores --------------------------------------------------
+ * For networks that are binary in part, e.g. heads and projections that keep 16-bit values.  No reference
+ * counterparts. */
+/* Element types, and activations: z, max(z, 0), z Phi(z), its tanh form, z / (1 + e^-z). */
+#define TCBNN_FP32 0
+#define TCBNN_FP16 1
+#define TCBNN_BF16 2
+#define TCBNN_NO_ACTIVATION 0
+#define TCBNN_RELU 1
+#define TCBNN_GELU 2
+#define TCBNN_GELU_TANH 3
+#define TCBNN_SILU 4
+/* out[m][n] = act(sum_k x[m][k] * W[n][k] + bias[n]) + residual[m][n], for M >= 0 rows of x and N, K >= 1.
+ * x [M][ldx] and W [N][ldw] are of `type` (fp16 or bf16), bias [N] (or NULL) of that type or fp32 (bias_type), residual [M][ldr]
+ * (or NULL) and out [M][ldo] of `type` or fp32 (out_type).  Leading dimensions count elements; what lies between rows is neither
+ * read nor written.  Sums, activation and residual are fp32, the result is rounded once.
+ * residual may be out itself (same pointer and leading dimension); otherwise out shares no memory with an input.
+ * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for operands whose rows do not all start on 16 bytes (they
+ * are copied to rows that do; 0 for others).  Calls that may run at the same time need workspaces of their own. */
+size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw);
+int tcbnn_linear(const void* x, const void* W, const void* bias, const void* residual, void* out, int M, int N, int K, long long ldx,
+                 long long ldw, long long ldr, long long ldo, int type, int out_type, int bias_type, int activation, void* workspace,
+                 size_t workspace_bytes, void* stream);
+/* The same with binary weights: out = act(scale[n] * sum_k x[m][k] * w[n][k] + bias[n]) + residual[m][n], w[n][k] = +-1 the packed
+ * bits of row n (tcbnn_pack_fc_weight; ldw in words, a multiple of 4, 16-byte aligned; bits behind element K may be anything),
+ * scale [N] fp32 or NULL for 1.  Workspace as above with W = NULL. */
+int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const void* bias, const void* residual, void* out, int M,
+                     int N, int K, long long ldx, long long ldw, long long ldr, long long ldo, int type, int out_type, int bias_type,
+                     int activation, void* workspace, size_t workspace_bytes, void* stream);
+/* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
+ *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
+ *                                            0 for a negative target (a row without one), NaN for one past V - 1
+ *   entropy[m]  = ln S - sum(e^d d) / S      or NULL
+ *   top_ids, top_logp [M][top]               the `top` largest logits (0 <= top <= 32, top <= V) in falling order, equal ones in
+ *                                            rising order of their tokens, and their log probabilities
+ * A logit of -inf rules its token out: it has no part in the sums and is no alternative; where fewer than `top` are left the ids
+ * are -1 and the log probabilities -inf.  A row with every token ruled out has entropy 0 and log probability -inf.  A row that
+ * holds NaN or +inf has NaN for all of them, except that rows without a target keep 0; NaN is no alternative.
+ * temperature: 1e-30 to 1e30. */
+int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, const void* targets, int target_bytes, float temperature,
+                    int top, float* logp, float* entropy, int64_t* top_ids, float* top_logp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

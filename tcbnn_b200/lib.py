@@ -91,8 +91,13 @@ SIGNATURES = {
     "tcbnn_mma_peak": (_I, [_I, _I, _I, C.POINTER(C.c_double)]),
     "tcbnn_wait_probe": (_I, [_I, C.POINTER(C.c_int)]),
     "tcbnn_conv_prefers_chunked_residual": (_I, [C.POINTER(ConvDesc)]),
+    "tcbnn_linear_workspace_bytes": (_SZ, [_P, _P, _I, _I, _I, _LL, _LL]),
+    "tcbnn_linear": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
+    "tcbnn_bit_linear": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
+    "tcbnn_log_probs": (_I, [_P, _I, _I, _I, _LL, _P, _I, C.c_float, _I, _P, _P, _P, _P, _P]),
 }
 
+FP32, FP16, BF16 = 0, 1, 2                                              # TCBNN_FP32, ...
 RES_INT32, RES_INT16, RES_INT16_CHUNKED, RES_PROVEN = 4, 2, 18, 32      # TCBNN_RES_* of the header
 
 _lib = None

@@ -596,6 +596,12 @@ class Network:
             p.seen = 2 if last is not None and not last.common.noted and last.input == p.input else 1
         return self.layers[-1].get_output_gpu()
 
+    def score(self, targets=None, top=0, temperature=1.0):
+        """Scores of the last pass's logits, those of the live images: (log probability of the given class, 0
+        where it is negative; entropy; the `top` likeliest classes; their log probabilities), see ops.log_probs."""
+        logits = self.layers[-1].get_output_gpu()
+        return ops.log_probs(logits if self.live_batch is None else logits[:self.live_batch], targets, top, temperature)
+
     MAX_GRAPHS = 16
 
     def forward_graph(self):

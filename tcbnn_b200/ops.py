@@ -167,6 +167,123 @@ def out_layer(A, W, scale, bias, K, out=None, workspace=None):
     return out
 
 
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+_TYPES = {torch.float32: _l.FP32, torch.float16: _l.FP16, torch.bfloat16: _l.BF16}
+
+
+def _rows(name, t, device, dtypes, width=None, rows=None):
+    """Leading dimension of a 2-d operand on the current device whose rows are contiguous."""
+    if not t.is_cuda:
+        raise _l.TcbnnError("tcbnn_b200 ops need CUDA tensors (no CPU path exists)")
+    if t.dim() != 2 or t.dtype not in dtypes or (width is not None and t.shape[1] != width) or (rows is not None and t.shape[0] != rows):
+        raise _l.TcbnnError(f"{name}: a tensor {[rows or 'rows', width or 'columns']} of {' or '.join(map(str, dtypes))} is wanted, "
+                            f"not {list(t.shape)} of {t.dtype}")
+    if t.get_device() != device:
+        raise _l.TcbnnError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
+    ld, inner = t.stride()
+    if inner != 1 and t.shape[1] != 1:
+        raise _l.TcbnnError(f"{name}: the elements of a row must be next to each other")
+    if t.shape[0] <= 1:
+        return max(ld, t.shape[1])
+    if ld < t.shape[1]:
+        raise _l.TcbnnError(f"{name}: rows overlap")
+    return ld
+
+
+def _vector(name, t, device, dtypes, n):
+    """Pointer of a vector of n on the current device, None without one."""
+    if t is None:
+        return None
+    if not t.is_cuda or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous() or t.get_device() != device:
+        raise _l.TcbnnError(f"{name}: a contiguous vector of {n} of {' or '.join(map(str, dtypes))} on cuda:{device} is wanted, "
+                            f"not {list(t.shape)} of {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+_REAL16, _WORDS, _FP32 = (torch.bfloat16, torch.float16), (torch.int32,), (torch.float32,)
+
+
+def _product(x, weight, scale, bias, activation, residual, out, out_dtype, workspace, bits):
+    device = _current_device()
+    xt = x.dtype
+    ldx = _rows("x", x, device, _REAL16)
+    M, K = x.shape
+    ldw = _rows("weight", weight, device, _WORDS if bits else (xt,), None if bits else K)
+    N = weight.shape[0]
+    if bits and weight.shape[1] * 32 < K:
+        raise _l.TcbnnError(f"weight: {weight.shape[1]} words do not hold {K} bits")
+    if activation not in ACTIVATIONS:
+        raise _l.TcbnnError(f"activation: one of {', '.join(ACTIVATIONS)} is wanted, not {activation!r}")
+    if out is not None:
+        out_dtype = out.dtype if out_dtype is None else out_dtype
+    elif out_dtype is None:
+        out_dtype = xt
+    if out_dtype is not xt and out_dtype is not torch.float32:
+        raise _l.TcbnnError(f"the result is of {xt} or torch.float32, not {out_dtype}")
+    ot = (out_dtype,)
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        ldo = N
+    else:
+        ldo = _rows("out", out, device, ot, N, M)
+    ldr = 0 if residual is None else _rows("residual", residual, device, ot, N, M)
+    bias_p = _vector("bias", bias, device, (xt, torch.float32), N)
+    need = 0 if M == 0 else _l.bound("tcbnn_linear_workspace_bytes")(x.data_ptr(), None if bits else weight.data_ptr(), M, N, K, ldx, ldw)
+    if workspace is None and need:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    sizes = (M, N, K, ldx, ldw, ldr, ldo, _TYPES[xt], _TYPES[out_dtype], _TYPES[xt if bias is None else bias.dtype],
+             ACTIVATIONS[activation], ws, ws_bytes, _raw_stream(device))
+    if bits:
+        _l.call("tcbnn_bit_linear", x.data_ptr(), weight.data_ptr(), _vector("scale", scale, device, _FP32, N), bias_p, _ptr(residual),
+                out.data_ptr(), *sizes)
+    else:
+        _l.call("tcbnn_linear", x.data_ptr(), weight.data_ptr(), bias_p, _ptr(residual), out.data_ptr(), *sizes)
+    return out
+
+
+def linear_workspace(x, weight):
+    """Scratch that linear() needs on these operands (bit_linear(): weight=None), or None; without one given it is
+    allocated per call."""
+    N, ldw = (1, 8) if weight is None else (weight.shape[0], weight.stride(0))
+    n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), _ptr(weight), x.shape[0], N, x.shape[1], max(x.stride(0), x.shape[1]), ldw)
+    return torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
+
+
+def linear(x, weight, bias=None, activation="none", residual=None, out=None, out_dtype=None, workspace=None):
+    """act(x @ weight.T + bias) + residual, sums in fp32, rounded once (tcbnn_linear).
+    x [M][K] and weight [N][K]: bf16 or fp16, rows contiguous, any distance apart; rows that start on multiples of 16 bytes are read
+    as they are, others copied first.  bias [N]: x's type or fp32.  residual [M][N] and out: x's type or fp32 (out_dtype); residual
+    may be out itself.  activation: "none", "relu", "gelu", "gelu_tanh" or "silu"."""
+    return _product(x, weight, None, bias, activation, residual, out, out_dtype, workspace, False)
+
+
+def bit_linear(x, weight, scale=None, bias=None, activation="none", residual=None, out=None, out_dtype=None, workspace=None):
+    """act(scale * (x @ w.T) + bias) + residual with binary weights: w[n][k] = +-1 the bits of row n of `weight`, int32 words as
+    pack_fc_weight() lays them out; scale [N] fp32 or None for 1 (tcbnn_bit_linear).  The rest as linear()."""
+    return _product(x, weight, scale, bias, activation, residual, out, out_dtype, workspace, True)
+
+
+def log_probs(logits, targets=None, top=0, temperature=1.0):
+    """(logp [M], entropy [M], top_ids [M][top], top_logp [M][top]) of logits [M][V] (fp32, fp16 or bf16, rows contiguous, any
+    distance apart) divided by `temperature` (tcbnn_log_probs).
+    logp: of the given tokens targets [M] (int32 or int64), 0 where that is negative; None without targets.  top_ids (int64): the `top`
+    likeliest tokens (at most 32), equal ones in rising order; -1 behind the last token whose logit is not -inf."""
+    device = _current_device()
+    ld = _rows("logits", logits, device, tuple(_TYPES))
+    M, V = logits.shape
+    targets_p = _vector("targets", targets, device, (torch.int64, torch.int32), M)
+    if not 0 <= top <= 32:
+        raise _l.TcbnnError(f"top must be between 0 and 32, not {top}")
+    where = dict(dtype=torch.float32, device=logits.device)
+    logp = None if targets is None else torch.empty((M,), **where)
+    entropy, top_logp = torch.empty((M,), **where), torch.empty((M, top), **where)
+    top_ids = torch.empty((M, top), dtype=torch.int64, device=logits.device)
+    _l.call("tcbnn_log_probs", logits.data_ptr(), _TYPES[logits.dtype], M, V, ld, targets_p, 0 if targets is None else targets.element_size(),
+            temperature, top, _ptr(logp), entropy.data_ptr(), top_ids.data_ptr(), top_logp.data_ptr(), _raw_stream(device))
+    return logp, entropy, top_ids, top_logp
+
+
 def conv_desc(B, H, W, Cc, O, R, S, stride_h=1, stride_w=1, padding=True, pool=1):
     d = ConvDesc(B=B, H=H, W=W, C=Cc, O=O, R=R, S=S, stride_h=stride_h, stride_w=stride_w,
                  padding=int(bool(padding)), pool=pool)
