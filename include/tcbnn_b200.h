@@ -420,6 +420,9 @@ int tcbnn_linear(const void* x, const void* W, const void* bias, const void* res
 int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const void* bias, const void* residual, void* out, int M,
                      int N, int K, long long ldx, long long ldw, long long ldr, long long ldo, int type, int out_type, int bias_type,
                      int activation, void* workspace, size_t workspace_bytes, void* stream);
+/* Device-side status word of these kernels, read as tcbnn_gemm_status reads its own (synchronises; 0 = fine, 1 = a bounded wait
+ * gave up and results since the last reading are not valid; reading a failure clears it). */
+int tcbnn_linear_status(int* status);
 /* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
  *                                            0 for a negative target (a row without one), NaN for one past V - 1

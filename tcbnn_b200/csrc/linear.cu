@@ -1,15 +1,26 @@
 // Kernels and C ABI of the products of real-valued rows (linear.cuh) and of the scores (log_probs.cuh).
 #include "../../include/tcbnn_b200.h"
 #include "host.cuh"
-#include "linear.cuh"
+#include "bnn_layers.cuh"
+#include "linear_umma.cuh"
 #include "log_probs.cuh"
 
 using namespace tcbnn;
 
 namespace {
 
-template <bool BITS>
-__global__ void __launch_bounds__(256) k_linear_64(linear::Args a) { linear::tile_64<BITS>(a); }
+__device__ int g_linear_status;      // 1 after a bounded wait inside k_linear gave up
+
+template <bool BITS, bool CLUSTER>
+__global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, 1)
+k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
+    extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
+    linear::umma_cta<BITS, CLUSTER>(a, p, &map_w, &map_x, status, dyn_smem_linear);
+}
+__global__ void __launch_bounds__(256) k_repack(const uint16_t* src, long long ld, int rows, int K, int pitch, uint16_t* dst) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product waits before it reads)
+    linear::repack(src, ld, rows, K, pitch, dst);
+}
 __global__ void __launch_bounds__(256) k_log_probs_row(scores::Args a) { scores::row(a); }
 
 size_t type_bytes(int type) { return type == TCBNN_FP32 ? 4 : 2; }
@@ -58,13 +69,112 @@ int check_linear(const char* what, const linear::Args& a, bool bits) {
     return 0;
 }
 
-int run_linear(const char* what, const linear::Args& a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+// Operands that tensor copies can read: rows that start on multiples of 16 bytes (less than 2^40 bytes apart)
+bool rows_fit(const void* p, long long ld, int rows) {
+    return ((uintptr_t)p & 15) == 0 && (rows == 1 || ((ld & 7) == 0 && ld < (1LL << 39)));
+}
+size_t packed_bytes(int rows, int K) { return ((size_t)rows * ((K + 7) & ~7) * 2 + 255) & ~(size_t)255; }
+
+// The plan with the least clocks.  A block of 64 of K costs a CTA its MMAs (cols / 2 each), its bytes from L2, or, with packed
+// weights, the expanders' time; a tile its set-up and what of the epilogue shows; a cluster its exchange.
+linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
+    linear::Plan best = {};
+    double least = 1e300;
+    const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
+    for (int splits = 1; splits <= 8; splits *= 2) {
+        const int per = ((kblocks + splits - 1) / splits + unit - 1) / unit * unit;
+        if (splits > 1 && (splits - 1) * per >= kblocks) continue;       // (a CTA without work)
+        const int clusters = splits == 1 ? sms : splits == 2 ? sms / 2 : splits == 4 ? sms * 33 / 148 : sms * 15 / 148;
+        for (int cols = 16; cols <= linear::kMaxCols; cols += 16) {
+            linear::Plan p = {};
+            p.cols = cols;
+            p.splits = splits;
+            p.tiles_m = (M + cols - 1) / cols;
+            p.tiles_n = (N + 127) / 128;
+            const long long tiles = (long long)p.tiles_m * p.tiles_n;
+            if (splits > 1 && tiles * splits > (1 << 20)) continue;
+            if (cols > 16 && p.tiles_m == 1 && cols >= M + 16) continue;
+            p.kblocks = kblocks;
+            p.per = per;
+            p.band = cols >= 128 ? 8 : 1024 / cols;
+            p.accumulators = tiles <= sms || (bits && cols > 192) ? 1 : 2;
+            p.ring = (512 - p.accumulators * cols) / 32;
+            if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
+            p.stages = (int)((226 * 1024 - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(cols, bits));
+            if (p.stages > linear::kMaxStages) p.stages = linear::kMaxStages;
+            if (linear::smem_bytes(p, bits) > 227 * 1024) continue;
+            const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + cols * 128.0;
+            double block = bytes / 72 > mma ? bytes / 72 : mma;
+            if (bits && block < 130) block = 130;
+            const double finish = 400 + cols * 12.0, waves = (double)((tiles + clusters - 1) / clusters);
+            const double clocks = waves * (p.per * block + (p.accumulators == 1 ? finish : 200)) + finish + 2500 + (splits > 1 ? 2000 : 0);
+            if (clocks < least) { least = clocks; best = p; }
+        }
+    }
+    return best;
+}
+
+int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int width, int rows, long long pitch_bytes, int box_x, int box_y,
+               CUtensorMapSwizzle swizzle) {
+    if (!tensor_encode()) return fail("linear: the driver has no cuTensorMapEncodeTiled");
+    if (rows == 1) pitch_bytes = ((long long)width * (type == CU_TENSOR_MAP_DATA_TYPE_UINT32 ? 4 : 2) + 15) & ~15LL;
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)pitch_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box_x, (cuuint32_t)box_y}, steps[2] = {1, 1};
+    const CUresult e = tensor_encode()(map, type, 2, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (e != CUDA_SUCCESS) return fail("linear: tensor map of %d rows of %d: error %d", rows, width, (int)e);
+    return 0;
+}
+
+template <bool BITS>
+int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const CUtensorMap& map_w, const CUtensorMap& map_x, cudaStream_t st) {
+    static bool done[64];
+    if (configure_once(done, [] {
+            const cudaError_t e = cudaFuncSetAttribute(k_linear<BITS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            return e != cudaSuccess ? e : cudaFuncSetAttribute(k_linear<BITS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+        })) return 1;
+    void* status = nullptr;
+    CUDA_TRY(cudaGetSymbolAddress(&status, g_linear_status));
+    const long long tiles = (long long)p.tiles_m * p.tiles_n;
+    const int threads = BITS ? linear::kThreadsBits : linear::kThreadsDense;
+    const size_t smem = linear::smem_bytes(p, BITS);
+    const cudaError_t e = p.splits == 1 ? launch_dependent(k_linear<BITS, false>, (unsigned)(tiles < sms ? tiles : sms), threads, smem, st, a, p,
+                                                           (int*)status, map_w, map_x)
+                                        : launch_dependent_cluster(k_linear<BITS, true>, (unsigned)(tiles * p.splits), p.splits, threads, smem, st,
+                                                                   a, p, (int*)status, map_w, map_x);
+    if (e != cudaSuccess) return fail("linear: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int run_linear(const char* what, linear::Args a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {
     if (check_linear(what, a, bits)) return 1;
     if (a.M == 0) return 0;
-    const dim3 grid((a.N + 63) / 64, (a.M + 63) / 64);
-    if (bits) k_linear_64<true><<<grid, 256, 0, st>>>(a);
-    else k_linear_64<false><<<grid, 256, 0, st>>>(a);
-    return launch_check(what);
+    int sms;
+    if (sm_count(&sms)) return 1;
+    const size_t need = tcbnn_linear_workspace_bytes(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
+    if (need) {
+        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
+            return fail("%s: these operands need %zu bytes of workspace, 256-byte aligned", what, need);
+        char* room = (char*)workspace;
+        const int pitch = (a.K + 7) & ~7;
+        auto repack = [&](const void** p, long long* ld, int rows) {
+            const long long units = (long long)rows * (pitch / 8), blocks = (units + 255) / 256;
+            k_repack<<<(unsigned)(blocks < 16LL * sms ? blocks : 16LL * sms), 256, 0, st>>>((const uint16_t*)*p, *ld, rows, a.K, pitch, (uint16_t*)room);
+            *p = room;
+            *ld = pitch;
+            room += packed_bytes(rows, a.K);
+        };
+        if (!rows_fit(a.x, a.ldx, a.M)) repack(&a.x, &a.ldx, a.M);
+        if (!bits && !rows_fit(a.W, a.ldw, a.N)) repack(&a.W, &a.ldw, a.N);
+        if (launch_check(what)) return 1;
+    }
+    const linear::Plan p = plan_linear(a.M, a.N, a.K, bits, sms);
+    const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap map_w, map_x;
+    if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, p.cols, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
+    if (bits ? linear_map(&map_w, a.W, CU_TENSOR_MAP_DATA_TYPE_UINT32, (a.K + 31) / 32, a.N, a.ldw * 4, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B)
+             : linear_map(&map_w, a.W, type, a.K, a.N, a.ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
+    return bits ? launch_linear<true>(a, p, sms, map_w, map_x, st) : launch_linear<false>(a, p, sms, map_w, map_x, st);
 }
 
 }  // namespace
@@ -72,8 +182,8 @@ int run_linear(const char* what, const linear::Args& a, bool bits, void* workspa
 extern "C" {
 
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw) {
-    (void)x; (void)W; (void)M; (void)N; (void)K; (void)ldx; (void)ldw;
-    return 0;
+    if (M < 1 || N < 1 || K < 1) return 0;
+    return (rows_fit(x, ldx, M) ? 0 : packed_bytes(M, K)) + (!W || rows_fit(W, ldw, N) ? 0 : packed_bytes(N, K));
 }
 
 int tcbnn_linear(const void* x, const void* W, const void* bias, const void* residual, void* out, int M, int N, int K, long long ldx,
@@ -81,6 +191,17 @@ int tcbnn_linear(const void* x, const void* W, const void* bias, const void* res
                  size_t workspace_bytes, void* stream) {
     const linear::Args a{x, W, nullptr, bias, residual, out, M, N, K, ldx, ldw, ldr, ldo, type, out_type, bias_type, activation};
     return run_linear("linear", a, false, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int tcbnn_linear_status(int* status) {
+    if (!status) return fail("linear_status: null pointer");
+    CUDA_TRY(cudaDeviceSynchronize());
+    CUDA_TRY(cudaMemcpyFromSymbol(status, g_linear_status, sizeof(int)));
+    if (*status) {                                       // reading a failure clears it
+        const int zero = 0;
+        CUDA_TRY(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)));
+    }
+    return 0;
 }
 
 int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const void* bias, const void* residual, void* out, int M, int N,

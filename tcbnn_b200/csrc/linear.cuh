@@ -1,8 +1,6 @@
 // Products of real-valued rows: y[m][n] = act(s[n] * sum_k x[m][k] * w[n][k] + b[n]) + r[m][n], x in bf16 or fp16,
 // w of the same type (s = 1) or packed signs of +-1 with a scale per output.  Sums, scale, bias, activation and
-// residual are fp32; the result is rounded once, to x's type or not at all.
-//
-// This form computes 64 x 64 outputs per block from shared memory with fp32 multiply-adds, any strides.
+// residual are fp32; the result is rounded once, to x's type or not at all.  Types, arguments and what happens to a sum.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -38,49 +36,6 @@ __device__ __forceinline__ float activate(float z, int a) {
     if (a == GELU_TANH) return 0.5f * z * (1.f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
     if (a == SILU) return z / (1.f + expf(-z));
     return z;
-}
-
-template <bool BITS>
-__device__ __forceinline__ void tile_64(const Args& a) {
-    __shared__ float sx[16][65], sw[16][65];
-    const int n0 = blockIdx.x * 64, m0 = blockIdx.y * 64, t = threadIdx.x, tn = t & 15, tm = t >> 4;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += 16) {
-        for (int i = t; i < 1024; i += 256) {
-            const int r = i >> 4, k = i & 15;
-            float x = 0.f, w = 0.f;
-            if (k0 + k < a.K) {
-                if (m0 + r < a.M) x = load(a.x, (m0 + r) * a.ldx + k0 + k, a.type);
-                if (n0 + r < a.N) {
-                    if (BITS) w = reinterpret_cast<const uint32_t*>(a.W)[(n0 + r) * a.ldw + ((k0 + k) >> 5)] >> (31 - ((k0 + k) & 31)) & 1u ? 1.f : -1.f;
-                    else w = load(a.W, (n0 + r) * a.ldw + k0 + k, a.type);
-                }
-            }
-            sx[k][r] = x;
-            sw[k][r] = w;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sx[k][tm + 16 * i], sw[k][tn + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int m = m0 + tm + 16 * i, n = n0 + tn + 16 * j;
-            if (m >= a.M || n >= a.N) continue;
-            float z = acc[i][j];
-            if (BITS && a.scale) z *= a.scale[n];
-            if (a.bias) z += load(a.bias, n, a.bias_type);
-            z = activate(z, a.activation);
-            if (a.residual) z += load(a.residual, m * a.ldr + n, a.out_type);
-            store(a.out, m * a.ldo + n, a.out_type, z);
-        }
 }
 
 }  // namespace linear

@@ -1,0 +1,409 @@
+// Products of real-valued rows on tcgen05 (kind::f16, fp32 accumulators in tensor memory):
+// y[m][n] = act(s[n] * sum_k x[m][k] w[n][k] + b[n]) + r[m][n].
+//
+// The MMA's 128 rows are rows of W (outputs), its columns rows of x (tokens): one token costs 16 columns, a prompt 256,
+// by the same kernel, and what belongs to an output -- scale, bias, where it is stored -- belongs to a lane.
+//
+//   warps 0-7   epilogue  : lane = output, 32 tokens at a time
+//   warp  8     loader W  : tensor copies of 128 rows x 64 (dense) or 128 rows x 512 bits (packed)
+//   warp  9     loader x  : tensor copies of `cols` rows x 64
+//   warp  10    MMA       : converged, elected lane; four MMAs of K = 16 per 64
+//   warps 12-19 expanders : (packed) two groups of four: signs to +-1 in tensor memory, where the MMA reads its W operand
+//
+// Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.  Packed weights cost a
+// sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port either.
+//
+// Where tiles of 128 x cols leave SMs idle, K is cut over a cluster's CTAs, whose sums meet in shared memory, in rank
+// order: the same result every time.
+#pragma once
+#include "bconv_umma_pre.cuh"
+#include "linear.cuh"
+
+namespace tcbnn {
+namespace linear {
+
+constexpr int kThreadsDense = 11 * 32, kThreadsBits = 20 * 32;
+constexpr int kMaxCols = 256, kMaxStages = 12, kMaxRing = 8, kRawStages = 3;
+constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 rows of 64 elements, of 512 bits
+
+struct Plan {
+    int cols, splits;                                  // tokens per tile (a multiple of 16), CTAs that share K
+    int tiles_m, tiles_n, band;                        // tiles of tokens and of outputs; token tiles worked on together
+    int kblocks, per;                                  // of 64; of a CTA
+    int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
+};
+__host__ __device__ inline uint32_t stage_bytes(int cols, bool bits) { return (bits ? 0u : kWStage) + (uint32_t)cols * 128u; }
+// ring (where the cluster's sums go afterwards), raw bits, barriers; 1 KB for its alignment
+__host__ __device__ inline size_t ring_bytes(const Plan& p, bool bits) {
+    const size_t ring = (size_t)p.stages * stage_bytes(p.cols, bits), sums = p.splits > 1 ? (size_t)p.cols * 512 : 0;
+    return ((ring > sums ? ring : sums) + 1023) & ~(size_t)1023;
+}
+__host__ __device__ inline size_t smem_bytes(const Plan& p, bool bits) {
+    return ring_bytes(p, bits) + (bits ? kRawStages * kRawStage : 0) + 64 * 8 + 1024;
+}
+
+__device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+// rows of 128 bytes, 128-byte swizzle, eight rows 1 KB apart from the next
+__device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp16 or bf16 operands, both K-major, fp32 sums, M = 128
+__device__ __forceinline__ uint32_t idesc_16(int type, int n) {
+    const uint32_t f = type == BF16 ? 1u : 0u;
+    return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// Four MMAs over 64 elements of K: both operands 32 bytes (two 16-byte units of the descriptor) on each time, or A
+// eight columns of tensor memory.
+__device__ __forceinline__ void mma_64(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+#define TCBNN_MMA(PRED)                                                                              \
+    "mov.b64 da, {xa, %4};\n\tmov.b64 db, {xb, %4};\n\t"                                            \
+    "@pl tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %5, " PRED ";\n\tadd.u32 xa, xa, 2;\n\tadd.u32 xb, xb, 2;\n\t"
+    asm volatile("{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 da, db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t"
+                 "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
+                 TCBNN_MMA("pa") TCBNN_MMA("pt") TCBNN_MMA("pt") TCBNN_MMA("pt") "}"
+                 ::"r"(leader), "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory");
+#undef TCBNN_MMA
+}
+__device__ __forceinline__ void mma_64_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+#define TCBNN_MMA(PRED)                                                                              \
+    "mov.b64 db, {xb, %4};\n\t"                                                                     \
+    "@pl tcgen05.mma.cta_group::1.kind::f16 [%1], [xa], db, %5, " PRED ";\n\tadd.u32 xa, xa, 8;\n\tadd.u32 xb, xb, 2;\n\t"
+    asm volatile("{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t"
+                 "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
+                 TCBNN_MMA("pa") TCBNN_MMA("pt") TCBNN_MMA("pt") TCBNN_MMA("pt") "}"
+                 ::"r"(leader), "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory");
+#undef TCBNN_MMA
+}
+// 32 signs as 16 pairs of +-1: register i holds elements 2i (low half) and 2i + 1, which are bits 31 - 2i and 30 - 2i.  `minus`:
+// -1 twice, whose signs a set bit turns.  The word is laid out once so that a shift brings both bits to their places.
+__device__ __forceinline__ void expand_signs(uint32_t w, uint32_t minus, uint32_t* r) {
+    const uint32_t a = __byte_perm(w, w << 1, 0x7632), b = __byte_perm(w, w << 1, 0x5410);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        r[i] = ((a << (2 * i)) & 0x80008000u) ^ minus;
+        r[8 + i] = ((b << (2 * i)) & 0x80008000u) ^ minus;
+    }
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&e)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+                 "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(e[0]), "r"(e[1]), "r"(e[2]), "r"(e[3]), "r"(e[4]), "r"(e[5]), "r"(e[6]), "r"(e[7]), "r"(e[8]), "r"(e[9]),
+                   "r"(e[10]), "r"(e[11]), "r"(e[12]), "r"(e[13]), "r"(e[14]), "r"(e[15]), "r"(e[16]), "r"(e[17]), "r"(e[18]), "r"(e[19]),
+                   "r"(e[20]), "r"(e[21]), "r"(e[22]), "r"(e[23]), "r"(e[24]), "r"(e[25]), "r"(e[26]), "r"(e[27]), "r"(e[28]), "r"(e[29]),
+                   "r"(e[30]), "r"(e[31]) : "memory");
+}
+__device__ __forceinline__ float4 ld_peer4(uint32_t shared, uint32_t rank) {
+    uint32_t p;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(p) : "r"(shared), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(p) : "memory");
+    return v;
+}
+
+// What a lane knows of its output, and how a sum becomes a result
+struct Output {
+    const Args& a;
+    int n;
+    float scale, bias;
+    __device__ __forceinline__ Output(const Args& a_, int n_) : a(a_), n(n_), scale(1.f), bias(0.f) {
+        if (n >= a.N) return;
+        if (a.scale) scale = ld_dep(a.scale + n);
+        if (a.bias) bias = load(a.bias, n, a.bias_type);
+    }
+    template <int COUNT>
+    __device__ __forceinline__ void finish(float (&v)[COUNT], int m0, int rows) const {
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) v[j] = fmaf(v[j], scale, bias);
+        switch (a.activation) {
+        case RELU:
+#pragma unroll
+            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], RELU);
+            break;
+        case GELU:
+#pragma unroll
+            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU);
+            break;
+        case GELU_TANH:
+#pragma unroll
+            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU_TANH);
+            break;
+        case SILU:
+#pragma unroll
+            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], SILU);
+            break;
+        }
+        if (n >= a.N) return;
+        if (a.residual) {
+#pragma unroll
+            for (int j = 0; j < COUNT; j++)
+                if (j < rows) v[j] += load(a.residual, (m0 + j) * a.ldr + n, a.out_type);
+        }
+#pragma unroll
+        for (int j = 0; j < COUNT; j++)
+            if (j < rows) store(a.out, (m0 + j) * a.ldo + n, a.out_type, v[j]);
+    }
+};
+
+template <bool BITS, bool CLUSTER>
+__device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUtensorMap* map_w, const CUtensorMap* map_x, int* status,
+                                         unsigned char* smem0) {
+    using namespace umma;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem0) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t nctas = CLUSTER ? [] { uint32_t n; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }() : 1u;
+    const uint32_t rank = CLUSTER ? [] { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }() : 0u;
+    const uint32_t stage = stage_bytes(p.cols, BITS);
+    unsigned char* sRaw = smem + ring_bytes(p, BITS);
+    uint64_t* sBar = reinterpret_cast<uint64_t*>(sRaw + (BITS ? kRawStages * kRawStage : 0));
+    // barriers: full[12] | empty[12] | ring full[8] | ring empty[8] | raw full[3] | raw empty[3] | sums full[2] | sums empty[2] | drain
+    uint32_t* sTmem = reinterpret_cast<uint32_t*>(sBar + 51);
+    volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
+    const uint32_t bar0 = smem_u32(sBar);
+    auto FULL = [&](int s) { return bar0 + 8u * s; };
+    auto EMPTY = [&](int s) { return bar0 + 8u * (12 + s); };
+    auto RFULL = [&](int s) { return bar0 + 8u * (24 + s); };
+    auto REMPTY = [&](int s) { return bar0 + 8u * (32 + s); };
+    auto RAWFULL = [&](int s) { return bar0 + 8u * (40 + s); };
+    auto RAWEMPTY = [&](int s) { return bar0 + 8u * (43 + s); };
+    auto SFULL = [&](int b) { return bar0 + 8u * (46 + b); };
+    auto SEMPTY = [&](int b) { return bar0 + 8u * (48 + b); };
+    const uint32_t DRAIN = bar0 + 8u * 50;
+
+    const int t_first = CLUSTER ? (int)(blockIdx.x / nctas) : (int)blockIdx.x, t_step = CLUSTER ? (int)(gridDim.x / nctas) : (int)gridDim.x;
+    const int ntiles = p.tiles_m * p.tiles_n;
+    const int kb0 = (int)rank * p.per, nkb = max(0, min(p.per, p.kblocks - kb0));     // this CTA's blocks of K
+    // bands of token tiles, in a band the tokens fastest: what runs together shares rows of both operands
+    auto tile = [&](int t, int& tm, int& tn) {
+        const int full = p.band * p.tiles_n, b = t / full, r = t - b * full, w = min(p.band, p.tiles_m - b * p.band);
+        tn = r / w;
+        tm = b * p.band + r - tn * w;
+    };
+
+    if (tid == 0) {
+        for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
+        for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), 4); mbar_init(REMPTY(s), 1); }
+        for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 8); }
+        for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), 8); }
+        mbar_init(DRAIN, 1);
+        *sAbort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 10) tmem_alloc(smem_u32(sTmem), 512);
+    fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *sTmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (not before the allocation: see bconv_umma_pre.cuh)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const WsWait wait{sAbort, status};
+    const uint32_t ring_col = (uint32_t)(p.accumulators * p.cols);
+
+    if (warp == 8 || warp == 9) {
+        // =============================== loaders ============================================
+        if (lane == 0 && nkb > 0) {
+            const bool isw = warp == 8;
+            const int step = BITS && isw ? 8 : 1, slots = BITS && isw ? kRawStages : p.stages;
+            int s = 0, issued = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int t = t_first; t < ntiles && ok; t += t_step) {
+                int tm, tn;
+                tile(t, tm, tn);
+                for (int kb = 0; kb < nkb; kb += step) {
+                    ok = wait(BITS && isw ? RAWEMPTY(s) : EMPTY(s), ph ^ 1);
+                    if (!ok) break;
+                    if (BITS && isw) {
+                        mbar_expect_tx(RAWFULL(s), kRawStage);
+                        tensor_g2s(smem_u32(sRaw) + s * kRawStage, map_w, (kb0 + kb) * 2, tn * 128, RAWFULL(s));
+                    } else {
+                        const uint32_t bytes = isw ? kWStage : (uint32_t)p.cols * 128u;
+                        mbar_expect_tx(FULL(s), bytes);
+                        tensor_g2s(smem_u32(smem) + s * stage + (isw || BITS ? 0u : kWStage), isw ? map_w : map_x, (kb0 + kb) * 64,
+                                   isw ? tn * 128 : tm * p.cols, FULL(s));
+                    }
+                    issued++;
+                    if (++s == slots) { s = 0; ph ^= 1; }
+                }
+            }
+            if (!ok) {
+                // giving up: wait (bounded) for the copies still in flight before the CTA exits
+                for (int s2 = 0; s2 < slots; s2++) {
+                    const bool this_pass = s2 < s;
+                    if (!this_pass && issued < slots) continue;
+                    for (int i = 0; i < (1 << 20); i++)
+                        if (mbar_try_wait(BITS && isw ? RAWFULL(s2) : FULL(s2), this_pass ? ph : ph ^ 1)) break;
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 10) {
+        // =============================== MMA issuer =========================================
+        const uint32_t leader = elect_one() ? 1u : 0u;
+        const uint32_t idesc = idesc_16(a.type, p.cols);
+        const uint64_t desc0 = swizzled_desc(smem_u32(smem));
+        const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
+        int s = 0, r = 0, b = 0;
+        uint32_t ph = 0, rph = 0, bph = 0;
+        bool ok = true;
+        if (nkb > 0)
+            for (int t = t_first; t < ntiles && ok; t += t_step) {
+                ok = wait.spin(SEMPTY(b), bph ^ 1);
+                if (!ok) break;
+                const uint32_t d = tmem + b * p.cols;
+                for (int kb = 0; kb < nkb; kb++) {
+                    if (BITS) ok = wait.spin(RFULL(r), rph);
+                    if (ok) ok = wait.spin(FULL(s), ph);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t lo = lo0 + (s * stage >> 4);
+                    if constexpr (BITS) mma_64_ts(leader, d, tmem + ring_col + r * 32, lo, hi, idesc, kb > 0);
+                    else mma_64(leader, d, lo, lo + (kWStage >> 4), hi, idesc, kb > 0);
+                    if (leader) {
+                        mma_commit(EMPTY(s));
+                        if (BITS) mma_commit(REMPTY(r));
+                        if (kb + 1 == nkb) mma_commit(SFULL(b));
+                    }
+                    __syncwarp();
+                    if (++s == p.stages) { s = 0; ph ^= 1; }
+                    if (BITS && ++r == p.ring) { r = 0; rph ^= 1; }
+                }
+                if (++b == p.accumulators) { b = 0; bph ^= 1; }
+            }
+        if (!ok && leader) {
+            // giving up: the MMAs already issued must have finished before tensor memory is freed
+            mma_commit(DRAIN);
+            for (int i = 0; i < (1 << 20); i++)
+                if (mbar_try_wait(DRAIN, 0)) break;
+        }
+        __syncwarp();
+    } else if (BITS && warp >= 12) {
+        // =============================== expanders ==========================================
+        const int group = (warp - 12) >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const uint32_t minus = a.type == BF16 ? 0xBF80BF80u : 0xBC00BC00u;
+        const uint32_t dst0 = tmem + ((uint32_t)(quad * 32) << 16) + ring_col;
+        int raw = 0, count = 0;                          // count: blocks of K in front, modulo two turns of the ring
+        uint32_t rawph = 0;
+        bool ok = true;
+        if (nkb > 0)
+            for (int t = t_first; t < ntiles && ok; t += t_step)
+                for (int kb = 0; kb < nkb && ok; kb += 8) {
+                    const int blocks = min(8, nkb - kb);
+                    ok = wait(RAWFULL(raw), rawph);
+                    if (!ok) break;
+                    // (the copy's 64-byte swizzle: 16-byte pieces turned by the row)
+                    const uint32_t src = smem_u32(sRaw) + raw * kRawStage + row * 64;
+                    for (int j = group; j < blocks; j += 2) {
+                        uint32_t w0, w1, e[32];
+                        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w0), "=r"(w1)
+                                     : "r"(src + (((j >> 1) ^ ((row >> 1) & 3)) << 4) + (j & 1) * 8) : "memory");
+                        expand_signs(w0, minus, e);
+                        expand_signs(w1, minus, e + 16);
+                        int at = count + j;
+                        if (at >= 2 * p.ring) at -= 2 * p.ring;
+                        const int r = at >= p.ring ? at - p.ring : at;
+                        ok = wait(REMPTY(r), at >= p.ring ? 0u : 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        tmem_st32(dst0 + r * 32, e);
+                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(RFULL(r));
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(RAWEMPTY(raw));
+                    count += blocks;
+                    if (count >= 2 * p.ring) count -= 2 * p.ring;
+                    if (++raw == kRawStages) { raw = 0; rawph ^= 1; }
+                }
+        __syncwarp();
+    } else if (warp < 8) {
+        // =============================== epilogue ===========================================
+        const int quad = warp & 3, half = warp >> 2;
+        int b = 0;
+        uint32_t bph = 0;
+        bool ok = true;
+        for (int t = t_first; t < ntiles && ok; t += t_step) {
+            int tm, tn;
+            tile(t, tm, tn);
+            const Output out(a, tn * 128 + quad * 32 + lane);
+            if (nkb > 0) ok = wait.relaxed(SFULL(b), bph);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + b * p.cols;
+            for (int c0 = half * 32; c0 < p.cols; c0 += 64) {
+                const int m0 = tm * p.cols + c0;
+                if (!CLUSTER && m0 >= a.M) break;
+                int v[32];
+                tmem_ld32(tcol + c0, v);
+                tmem_ld_wait();
+                float f[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) f[j] = nkb > 0 ? __int_as_float(v[j]) : 0.f;
+                if constexpr (CLUSTER) {
+                    // sums for the cluster: [four columns][128 outputs][4]
+                    float4* dst = reinterpret_cast<float4*>(smem) + (size_t)(c0 >> 2) * 128 + quad * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (c0 + 4 * j < p.cols) dst[j * 128] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                } else {
+                    out.finish(f, m0, min(min(32, p.cols - c0), a.M - m0));
+                }
+            }
+            tc_fence_before();                           // this warp is done with the sums
+            __syncwarp();
+            if (lane == 0) mbar_arrive(SEMPTY(b));
+            if (++b == p.accumulators) { b = 0; bph ^= 1; }
+        }
+    }
+    tc_fence_before();
+    if constexpr (CLUSTER) {
+        // One tile per cluster: every CTA finishes each nctas-th group of four columns.
+        cluster_sync();
+        if (warp < 8 && !*sAbort) {
+            const int quad = warp & 3, half = warp >> 2;
+            int tm, tn;
+            tile(t_first, tm, tn);
+            const Output out(a, tn * 128 + quad * 32 + lane);
+            const int cols = min(p.cols, a.M - tm * p.cols);
+            const uint32_t src = smem_u32(smem) + (uint32_t)(quad * 32 + lane) * 16u;
+            for (int c = 4 * ((int)rank + half * (int)nctas); c < cols; c += 8 * (int)nctas) {
+                float4 part[8];
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++)
+                    if (r < nctas) part[r] = ld_peer4(src + (uint32_t)c * 512u, r);
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (uint32_t r = 0; r < 8; r++)
+                    if (r < nctas) { v[0] += part[r].x; v[1] += part[r].y; v[2] += part[r].z; v[3] += part[r].w; }
+                out.finish(v, tm * p.cols + c, min(4, cols - c));
+            }
+            __syncwarp();
+        }
+        cluster_sync();                                  // nobody reads this CTA's sums any more
+    }
+    __syncthreads();
+    if (warp == 10) tmem_dealloc(tmem, 512);
+}
+
+// Rows of K elements of 16 bits, any distance apart, to rows of `pitch` elements
+__device__ __forceinline__ void repack(const uint16_t* src, long long ld, int rows, int K, int pitch, uint16_t* dst) {
+    const long long total = (long long)rows * (pitch / 8);
+    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
+        const long long r = i / (pitch / 8);
+        const int k = (int)(i - r * (pitch / 8)) * 8;
+        const uint16_t* s = src + r * ld + k;
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            w[j] = (k + 2 * j < K ? (uint32_t)s[2 * j] : 0u) | (k + 2 * j + 1 < K ? (uint32_t)s[2 * j + 1] << 16 : 0u);
+        reinterpret_cast<uint4*>(dst + r * pitch + k)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+}  // namespace linear
+}  // namespace tcbnn

@@ -264,6 +264,12 @@ def bit_linear(x, weight, scale=None, bias=None, activation="none", residual=Non
     return _product(x, weight, scale, bias, activation, residual, out, out_dtype, workspace, True)
 
 
+def linear_status():
+    s = C.c_int(0)
+    _l.call("tcbnn_linear_status", C.byref(s))
+    return s.value
+
+
 def log_probs(logits, targets=None, top=0, temperature=1.0):
     """(logp [M], entropy [M], top_ids [M][top], top_logp [M][top]) of logits [M][V] (fp32, fp16 or bf16, rows contiguous, any
     distance apart) divided by `temperature` (tcbnn_log_probs).
