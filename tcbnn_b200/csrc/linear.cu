@@ -1,5 +1,6 @@
 // Kernels and C ABI of the products of real-valued rows (linear.cuh) and of the scores (log_probs.cuh).
 #include "../../include/tcbnn_b200.h"
+#include <cmath>
 #include "host.cuh"
 #include "bnn_layers.cuh"
 #include "linear_umma.cuh"
@@ -21,7 +22,22 @@ __global__ void __launch_bounds__(256) k_repack(const uint16_t* src, long long l
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product waits before it reads)
     linear::repack(src, ld, rows, K, pitch, dst);
 }
-__global__ void __launch_bounds__(256) k_log_probs_row(scores::Args a) { scores::row(a); }
+template <int TYPE, int NW, bool CLUSTER>
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32, NW == 1 ? 4 : 32 / NW) k_log_probs(scores::Args a) {
+    __shared__ scores::Shared<NW> shared[NW == 1 ? 8 : 1];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if constexpr (CLUSTER) {
+        uint32_t n, r;
+        asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+        asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+        scores::row<TYPE, NW, true>(a, shared[0], blockIdx.x / n, r, n);
+    } else {
+        const int warp = NW == 1 ? threadIdx.x >> 5 : 0;
+        const long long r = NW == 1 ? blockIdx.x * 8LL + warp : blockIdx.x;
+        if (r < a.M) scores::row<TYPE, NW, false>(a, shared[warp], r, 0, 1);
+    }
+}
 
 size_t type_bytes(int type) { return type == TCBNN_FP32 ? 4 : 2; }
 
@@ -75,6 +91,8 @@ bool rows_fit(const void* p, long long ld, int rows) {
 }
 size_t packed_bytes(int rows, int K) { return ((size_t)rows * ((K + 7) & ~7) * 2 + 255) & ~(size_t)255; }
 
+int g_linear_cols = 0, g_linear_splits = 0;              // tcbnn_set_linear_plan: 0 = from the model
+
 // The plan with the least clocks.  A block of 64 of K costs a CTA its MMAs (cols / 2 each), its bytes from L2, or, with packed
 // weights, the expanders' time; a tile its set-up and what of the epilogue shows; a cluster its exchange.
 linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
@@ -82,8 +100,9 @@ linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
     for (int splits = 1; splits <= 8; splits *= 2) {
+        if (g_linear_splits && splits != g_linear_splits) continue;
         const int per = ((kblocks + splits - 1) / splits + unit - 1) / unit * unit;
-        if (splits > 1 && (splits - 1) * per >= kblocks) continue;       // (a CTA without work)
+        if (splits > 1 && (splits - 1) * per >= kblocks && !g_linear_splits) continue;       // (a CTA without work)
         const int clusters = splits == 1 ? sms : splits == 2 ? sms / 2 : splits == 4 ? sms * 33 / 148 : sms * 15 / 148;
         for (int cols = 16; cols <= linear::kMaxCols; cols += 16) {
             linear::Plan p = {};
@@ -93,7 +112,7 @@ linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
             p.tiles_n = (N + 127) / 128;
             const long long tiles = (long long)p.tiles_m * p.tiles_n;
             if (splits > 1 && tiles * splits > (1 << 20)) continue;
-            if (cols > 16 && p.tiles_m == 1 && cols >= M + 16) continue;
+            if (g_linear_cols ? cols != g_linear_cols : cols > 16 && cols >= M + 16) continue;
             p.kblocks = kblocks;
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
@@ -177,6 +196,30 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     return bits ? launch_linear<true>(a, p, sms, map_w, map_x, st) : launch_linear<false>(a, p, sms, map_w, map_x, st);
 }
 
+// How many warps share a row.  A warp's list holds 256 keys: it takes rows of up to eight batches of which no more than half as many are
+// expected to reach the bound, the top-th of 32 maxima over `per` logits each; 16 warps take rows that give every thread two batches, or
+// fewer where rows are few; beyond that the CTAs of a cluster, while every thread finds a batch.
+template <int TYPE>
+int run_log_probs(const scores::Args& a, int sms, cudaStream_t st) {
+    const int per = 4 * scores::Element<TYPE>::kPer;
+    const long long batches = (a.V + 32LL * per - 1) / (32 * per), want = 32LL * sms / a.M;
+    const double reach = a.top ? -log(1 - (a.top < 32 ? a.top : 31.5) / 32.0) / per * a.V : 0;
+    if ((batches < 4 || (batches <= 8 && want < 2)) && (reach <= 128 || a.V <= scores::kList1)) {
+        const unsigned grid = (unsigned)((a.M + 7LL) / 8);
+        const cudaError_t e = launch_dependent(k_log_probs<TYPE, 1, false>, grid, 256, 0, st, a);
+        return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
+    }
+    if (batches < 16 || (batches < 32 && want < 8)) {
+        const cudaError_t e = launch_dependent(k_log_probs<TYPE, 4, false>, (unsigned)a.M, 128, 0, st, a);
+        return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
+    }
+    unsigned ctas = 1;
+    while (ctas < 8 && batches >= 32LL * ctas && want >= 32LL * ctas) ctas *= 2;
+    const cudaError_t e = ctas == 1 ? launch_dependent(k_log_probs<TYPE, 16, false>, (unsigned)a.M, 512, 0, st, a)
+                                    : launch_dependent_cluster(k_log_probs<TYPE, 16, true>, (unsigned)a.M * ctas, ctas, 512, 0, st, a);
+    return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -191,6 +234,14 @@ int tcbnn_linear(const void* x, const void* W, const void* bias, const void* res
                  size_t workspace_bytes, void* stream) {
     const linear::Args a{x, W, nullptr, bias, residual, out, M, N, K, ldx, ldw, ldr, ldo, type, out_type, bias_type, activation};
     return run_linear("linear", a, false, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int tcbnn_set_linear_plan(int cols, int splits) {
+    if (cols < 0 || cols > linear::kMaxCols || cols % 16 || splits < 0 || splits > 8 || (splits & (splits - 1)))
+        return fail("set_linear_plan: cols is 0 or a multiple of 16 up to 256, splits is 0, 1, 2, 4 or 8");
+    g_linear_cols = cols;
+    g_linear_splits = splits;
+    return 0;
 }
 
 int tcbnn_linear_status(int* status) {
@@ -226,8 +277,11 @@ int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, co
         return fail("log_probs: a pointer is not aligned to its type");
     const scores::Args a{logits, targets, M, V, type, target_bytes, top, ld, 1.f / temperature, targets ? logp : nullptr, entropy,
                          (long long*)top_ids, top_logp};
-    k_log_probs_row<<<M, 256, 0, (cudaStream_t)stream>>>(a);
-    return launch_check("log_probs");
+    int sms;
+    if (sm_count(&sms)) return 1;
+    return type == TCBNN_FP32 ? run_log_probs<linear::FP32>(a, sms, (cudaStream_t)stream)
+         : type == TCBNN_FP16 ? run_log_probs<linear::FP16>(a, sms, (cudaStream_t)stream)
+                              : run_log_probs<linear::BF16>(a, sms, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -4,7 +4,15 @@
 // -inf and entropy 0; one that holds NaN or +inf has NaN for both.  Alternatives are ordered by (logit, lowest token),
 // NaN taking no part.
 //
-// This form reads a row once per block for the sums and once for every alternative.
+// One pass over the row.  A thread keeps the maximum m, s = sum e^{(x-m)/T} and t = sum e^{(x-m)/T} (x-m) of what it has seen; a
+// batch of 64 bytes that raises m rescales both once.  The alternatives are kept by a threshold: of the threads' maxima of the
+// first batch the top-th largest (of the two best per warp) is a bound that at least `top` logits reach; what reaches it
+// goes to a list in shared memory (a few hundred of 100,000 logits in random order), which is sorted at the end, 32 keys
+// to a warp, and merged.  Where the list overflows -- logits in rising order, or more ties than it holds -- the row is read
+// again, the list cut to its best `top` as often as it fills.
+//
+// A warp, 4 or 16 of them share a row, or the CTAs of a cluster, whose parts meet in the first one's shared memory.
+// Bound: HBM; 16-bit logits at 6.46 TB/s are 3.2e12 exponentials a second, 0.7 of what the units for them do.
 #pragma once
 #include "linear.cuh"
 
@@ -37,61 +45,350 @@ __device__ __forceinline__ int token_of(unsigned long long key) { return (int)(0
 
 // max m, sum e^{(x-m)/T} and sum e^{(x-m)/T} (x-m) of part of a row
 struct Sums { float m, s, t; };
-__device__ __forceinline__ void add(Sums& a, const Sums& b, float inv_t) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) { a.s += b.s; a.t += b.t; return; }              // (0, or NaN)
-    // a part far below m has nothing to add, whatever its distance times its sums comes to (fp32's lowest as a mask)
-    const float da = a.m - m, db = b.m - m, ea = expf(da * inv_t), eb = expf(db * inv_t);
-    a.t = (ea == 0.f ? 0.f : ea * fmaf(a.s, da, a.t)) + (eb == 0.f ? 0.f : eb * fmaf(b.s, db, b.t));
-    a.s = ea * a.s + eb * b.s;
-    a.m = m;
+
+constexpr int kList1 = 256, kList = 2048;              // keys that a row's list holds: of a warp, of several
+constexpr uint32_t kAll = 0xffffffffu;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// order of finite values and infinities as unsigned numbers, NaN and -inf lowest
+__device__ __forceinline__ uint32_t order_of(float x) { return (uint32_t)(key_of(x, 0) >> 32); }
+
+__device__ __forceinline__ uint4 load16(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+template <int TYPE>
+struct Element {
+    static constexpr int kBytes = TYPE == linear::FP32 ? 4 : 2, kPer = 16 / kBytes;
+    // element j of a vector
+    static __device__ __forceinline__ float get(const uint4& v, int j) {
+        if constexpr (TYPE == linear::FP32) {
+            return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w);
+        } else {
+            const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+            if constexpr (TYPE == linear::BF16) return __uint_as_float(j & 1 ? w & 0xFFFF0000u : w << 16);
+            else return __half2float(__ushort_as_half((unsigned short)(j & 1 ? w >> 16 : w & 0xFFFFu)));
+        }
+    }
+};
+
+// ---- sorted lists of 32 keys, one per lane, falling -------------------------------------------------
+__device__ __forceinline__ void exchange(unsigned long long& key, int distance, bool larger) {
+    const unsigned long long o = __shfl_xor_sync(kAll, key, distance);
+    if ((o > key) == larger) key = o;
+}
+__device__ __forceinline__ unsigned long long sort32(unsigned long long key) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int d = size / 2; d; d /= 2) exchange(key, d, ((lane & d) == 0) == ((lane & size) == 0));
+    return key;
+}
+// the 32 best of two falling lists (`other` given in rising order)
+__device__ __forceinline__ unsigned long long merge32(unsigned long long key, unsigned long long other) {
+    const int lane = threadIdx.x & 31;
+    if (other > key) key = other;
+#pragma unroll
+    for (int d = 16; d; d /= 2) exchange(key, d, (lane & d) == 0);
+    return key;
 }
 
-__device__ __forceinline__ void row(const Args& a) {
-    __shared__ Sums ss[256];
-    __shared__ unsigned long long sk[256];
-    const int r = blockIdx.x, t = threadIdx.x;
-    const long long base = r * a.ld;
-    Sums q{-INFINITY, 0.f, 0.f};
-    for (int i = t; i < a.V; i += 256) {
-        const float x = linear::load(a.logits, base + i, a.type);
-        if (x != -INFINITY) add(q, Sums{x, x == x && x != INFINITY ? 1.f : NAN, 0.f}, a.inv_t);
+template <int NW>
+struct Shared {
+    unsigned long long list[NW == 1 ? kList1 : kList];
+    unsigned long long best[NW == 1 ? 1 : 16][32];     // per warp; [0]: the row's
+    Sums sums[16];
+    uint32_t maxima[32];
+    uint32_t threshold;
+    int count;
+    unsigned long long cut;                            // of the second reading: what does not exceed it is out
+};
+template <int NW>
+__device__ __forceinline__ void meet() {
+    if constexpr (NW == 1) __syncwarp();
+    else __syncthreads();
+}
+
+// the 32 best of the first `n` of the list, falling, in the lanes of warp 0 (and in s.best[0])
+template <int NW>
+__device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n, int warp, int lane) {
+    unsigned long long key = 0;
+    for (int i = warp * 32; i < n; i += NW * 32) {
+        const unsigned long long other = sort32(i + lane < n ? s.list[i + lane] : 0ull);
+        key = merge32(key, __shfl_xor_sync(kAll, other, 31));
     }
-    ss[t] = q;
-    __syncthreads();
-    for (int h = 128; h; h >>= 1) {
-        if (t < h) add(ss[t], ss[t + h], a.inv_t);
+    if constexpr (NW > 1) {
+        const int lists = min(NW, (n + 31) >> 5);
+        s.best[warp][lane] = key;
         __syncthreads();
-    }
-    const Sums all = ss[0];
-    const float lse = logf(all.s);
-    auto logp = [&](float x) { return x == -INFINITY ? (all.s == all.s ? -INFINITY : NAN) : fmaf(x - all.m, a.inv_t, -lse); };
-    if (t == 0) {
-        const bool none = all.m == -INFINITY && all.s == 0.f;
-        if (a.logp) {
-            const long long y = !a.targets ? -1 : a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
-            a.logp[r] = y < 0 ? 0.f : y >= a.V ? NAN : logp(linear::load(a.logits, base + y, a.type));
-        }
-        if (a.entropy) a.entropy[r] = none ? 0.f : lse - all.t / all.s * a.inv_t;
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.top; k++) {
-        unsigned long long best = 0;
-        for (int i = t; i < a.V; i += 256) {
-            const unsigned long long key = key_of(linear::load(a.logits, base + i, a.type), i);
-            if (key < last && key > best) best = key;
-        }
-        __syncthreads();
-        sk[t] = best;
-        __syncthreads();
-        for (int h = 128; h; h >>= 1) {
-            if (t < h && sk[t + h] > sk[t]) sk[t] = sk[t + h];
+        for (int h = NW / 2; h; h /= 2) {
+            if (warp < h && warp + h < lists) s.best[warp][lane] = key = merge32(key, s.best[warp + h][31 - lane]);
             __syncthreads();
         }
-        last = sk[0];
-        if (t == 0) {
-            a.top_ids[(long long)r * a.top + k] = last ? token_of(last) : -1;
-            a.top_logp[(long long)r * a.top + k] = logp(last ? logit_of(last) : -INFINITY);
+    }
+    return key;
+}
+
+__device__ __forceinline__ void reduce(Sums& q, float c) {                // over a warp
+    const float m = logit_of((unsigned long long)__reduce_max_sync(kAll, order_of(q.m)) << 32);
+    const uint32_t any = __reduce_max_sync(kAll, order_of(q.m));
+    if (any) {                                         // (0: nothing but -inf so far; sums are 0, or NaN)
+        const float d = q.m - m, f = ex2(d * c);
+        q.t = f == 0.f ? (q.s == q.s ? 0.f : q.s) : f * fmaf(q.s, d, q.t);
+        q.s = f == 0.f && q.s == q.s ? 0.f : f * q.s;
+        q.m = m;
+    }
+#pragma unroll
+    for (int h = 16; h; h /= 2) {
+        q.s += __shfl_xor_sync(kAll, q.s, h);
+        q.t += __shfl_xor_sync(kAll, q.t, h);
+    }
+}
+
+template <int TYPE, int NW, bool CLUSTER>
+__device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, uint32_t rank, uint32_t nctas) {
+    using E = Element<TYPE>;
+    constexpr int THREADS = NW * 32, PER = E::kPer, U = 4, LIST = NW == 1 ? kList1 : kList;
+    const int tid = NW == 1 ? threadIdx.x & 31 : threadIdx.x, lane = tid & 31, warp = NW == 1 ? 0 : tid >> 5;
+    const char* base = reinterpret_cast<const char*>(a.logits) + r * a.ld * E::kBytes;
+    // elements in front of the first 16-byte boundary, vectors, elements behind them
+    const int head = min(a.V, (int)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / E::kBytes);
+    const int vectors = (a.V - head) / PER, tail = a.V - head - vectors * PER;
+    const char* body = base + head * E::kBytes;
+    const int v0 = CLUSTER ? (int)((long long)vectors * rank / nctas) : 0, v1 = CLUSTER ? (int)((long long)vectors * (rank + 1) / nctas) : vectors;
+    const bool first = rank == 0, last = rank + 1 == nctas;
+    const float c = a.inv_t * 1.44269504088896341f;    // log2 e / T
+
+    if (tid == 0) { s.count = 0; s.cut = 0; }
+    Sums q{-INFINITY, 0.f, 0.f};
+    float thr = -INFINITY;
+    auto add_max = [&](float bm) {                     // a batch's maximum
+        if (bm > q.m) {
+            if (q.m != -INFINITY) {
+                const float d = q.m - bm, f = ex2(d * c);
+                q.t = f == 0.f ? (q.t == q.t ? 0.f : q.t) : f * fmaf(q.s, d, q.t);
+                q.s *= f;
+            }
+            q.m = bm;
+        }
+    };
+    auto add_one = [&](float x, float m) {
+        const float d = x - m, e = ex2(d * c);
+        q.s += e;
+        q.t = fmaf(e, fmaxf(d, -3.0e38f), q.t);
+    };
+    auto push = [&](float x, int token) {
+        const unsigned long long key = key_of(x, token);
+        if (key) {
+            const int at = atomicAdd(&s.count, 1);
+            if (at < LIST) s.list[at] = key;
+        }
+    };
+    auto batch = [&](const uint4 (&v)[U], int i0) {    // vectors i0 + u * THREADS of the body
+        float bm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PER; j++) bm = fmaxf(bm, E::get(v[u], j));
+        add_max(bm);
+        const float m = q.m == -INFINITY ? 0.f : q.m;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PER; j++) add_one(E::get(v[u], j), m);
+        return bm;
+    };
+    auto push_batch = [&](const uint4 (&v)[U], int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < PER; j++) {
+                const float x = E::get(v[u], j);
+                if (x >= thr) push(x, head + (i0 + u * THREADS) * PER + j);
+            }
+    };
+    // (-inf: no part in anything)
+    const uint32_t fill = TYPE == linear::FP32 ? 0xFF800000u : TYPE == linear::BF16 ? 0xFF80FF80u : 0xFC00FC00u;
+    auto load = [&](uint4 (&v)[U], int i0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = i0 + u * THREADS < v1 ? load16(body + (long long)(i0 + u * THREADS) * 16) : make_uint4(fill, fill, fill, fill);
+    };
+
+    uint4 cur[U], next[U];
+    int i0 = v0 + tid;
+    load(cur, i0);
+    load(next, i0 + U * THREADS);
+    float bm = batch(cur, i0);
+    if (a.top) {
+        uint32_t o = order_of(bm);
+        if constexpr (NW == 1) {
+            // the top-th largest of 32 maxima
+            int more = 0;
+#pragma unroll
+            for (int i = 0; i < 32; i++) more += __shfl_sync(kAll, o, i) >= o;
+            o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
+        } else {
+            constexpr int BEST = 32 / NW;              // per warp: 2 of 16, 8 of 4
+            for (int i = 0; i < BEST; i++) {
+                const uint32_t most = __reduce_max_sync(kAll, o);
+                if (lane == 0) s.maxima[warp * BEST + i] = most;
+                if (lane == __ffs(__ballot_sync(kAll, o == most)) - 1) o = 0;
+            }
+            __syncthreads();
+            o = s.maxima[lane];
+            int more = 0;
+#pragma unroll
+            for (int i = 0; i < 32; i++) more += s.maxima[i] >= o;
+            o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
+        }
+        thr = o ? logit_of((unsigned long long)o << 32) : -INFINITY;
+        if (NW == 1) __syncwarp();                     // (the count is 0)
+        if (bm >= thr) push_batch(cur, i0);
+    }
+    const int batches = (v1 - v0 + U * THREADS - 1) / (U * THREADS);     // (of every thread: the last ones may find nothing)
+    for (int b = 1; b < batches; b++) {
+        i0 += U * THREADS;
+#pragma unroll
+        for (int u = 0; u < U; u++) cur[u] = next[u];
+        load(next, i0 + U * THREADS);
+        bm = batch(cur, i0);
+        if (a.top && bm >= thr) push_batch(cur, i0);
+        if (NW > 1 && a.top && (b & 3) == 3) {
+            // a list that is half full gives a better bound, and room
+            __syncthreads();
+            const int n = s.count;
+            __syncthreads();
+            if (n > LIST / 2 && n <= LIST) {
+                const unsigned long long best = best_of_list<NW>(s, n, warp, lane);
+                if (warp == 0) {
+                    if (lane < a.top) s.list[lane] = best;
+                    if (lane == a.top - 1) s.cut = best;
+                    if (lane == 0) s.count = a.top;
+                }
+                __syncthreads();
+                thr = logit_of(s.cut);
+            }
+        }
+    }
+    // the ends: a thread each
+    {
+        int at = -1;
+        if (first && tid < head) at = tid;
+        else if (last && tid >= 16 && tid - 16 < tail) at = head + vectors * PER + tid - 16;
+        if (at >= 0) {
+            const float x = linear::load(base, at, TYPE);
+            add_max(x);
+            add_one(x, q.m == -INFINITY ? 0.f : q.m);
+            if (a.top && x >= thr) push(x, at);
+        }
+    }
+    // sums of the row
+    reduce(q, c);
+    if constexpr (NW > 1) {
+        if (lane == 0) s.sums[warp] = q;
+        __syncthreads();
+        q = lane < NW ? s.sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+        reduce(q, c);
+    } else {
+        __syncwarp();
+    }
+    // alternatives
+    unsigned long long key = 0;
+    if (a.top) {
+        const int n = s.count;
+        if (n <= LIST) {
+            key = best_of_list<NW>(s, n, warp, lane);
+        } else {
+            // again, in short steps behind each of which the list has room for the next
+            const int from = first ? 0 : head + v0 * PER, to = last ? a.V : head + v1 * PER;
+            meet<NW>();
+            if (tid == 0) { s.count = 0; s.cut = 0; }
+            meet<NW>();
+            for (int e0 = from; e0 < to; e0 += 2 * THREADS) {
+                const unsigned long long cut = s.cut;
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const int e = e0 + j * THREADS + tid;
+                    const unsigned long long k = e < to ? key_of(linear::load(base, e, TYPE), e) : 0ull;
+                    if (k > cut) s.list[atomicAdd(&s.count, 1)] = k;
+                }
+                meet<NW>();
+                const int have = s.count;
+                meet<NW>();                            // (everybody has read it before it changes)
+                if (have > LIST - 2 * THREADS || e0 + 2 * THREADS >= to) {
+                    key = best_of_list<NW>(s, have, warp, lane);
+                    meet<NW>();
+                    if (warp == 0) {
+                        if (lane < a.top) s.list[lane] = key;
+                        if (lane == a.top - 1) s.cut = key;
+                        if (lane == 0) s.count = min(have, a.top);
+                    }
+                    meet<NW>();
+                }
+            }
+        }
+    }
+    if constexpr (CLUSTER) {
+        // the first CTA's first warp takes the others' parts
+        if (warp == 0) {
+            s.best[0][lane] = key;
+            if (lane == 0) s.sums[0] = q;
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (first) {
+            auto peer = [&](const void* p, uint32_t of) {
+                uint32_t x;
+                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(x) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(of));
+                return x;
+            };
+            auto ld = [&](uint32_t at) {
+                float v;
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                return v;
+            };
+            if (warp == 0) {
+                q = Sums{-INFINITY, 0.f, 0.f};
+                if ((uint32_t)lane < nctas) {
+                    const uint32_t at = peer(&s.sums[0], lane);
+                    q = Sums{ld(at), ld(at + 4), ld(at + 8)};
+                }
+                reduce(q, c);
+            }
+            if (a.top) {                               // warp w has the list of CTA w
+                if (warp > 0 && (uint32_t)warp < nctas)
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(peer(&s.best[0][lane], warp)) : "memory");
+                if ((uint32_t)warp < nctas) s.best[warp][lane] = key;
+                __syncthreads();
+                for (int h = (int)nctas / 2; h; h /= 2) {
+                    if (warp < h) s.best[warp][lane] = key = merge32(key, s.best[warp + h][31 - lane]);
+                    __syncthreads();
+                }
+            }
+        }
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (!first) return;
+    }
+    if (warp == 0) {
+        const float lse = logf(q.s);
+        auto logp = [&](float x) { return x == -INFINITY ? (q.s == q.s ? -INFINITY : q.s) : fmaf(x - q.m, a.inv_t, -lse); };
+        if (lane == 0) {
+            if (a.logp) {
+                const long long y = a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
+                a.logp[r] = y < 0 ? 0.f : y >= a.V ? NAN : logp(linear::load(base, y, TYPE));
+            }
+            if (a.entropy) a.entropy[r] = q.m == -INFINITY && q.s == 0.f ? 0.f : lse - q.t / q.s * a.inv_t;
+        }
+        if (lane < a.top) {
+            a.top_ids[r * a.top + lane] = key ? token_of(key) : -1;
+            a.top_logp[r * a.top + lane] = logp(key ? logit_of(key) : -INFINITY);
         }
     }
 }

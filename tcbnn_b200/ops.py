@@ -264,6 +264,11 @@ def bit_linear(x, weight, scale=None, bias=None, activation="none", residual=Non
     return _product(x, weight, scale, bias, activation, residual, out, out_dtype, workspace, True)
 
 
+def set_linear_plan(cols=0, splits=0):
+    """Force the tokens per tile and the CTAs that share K of linear() and bit_linear(); 0 = automatic."""
+    _l.call("tcbnn_set_linear_plan", int(cols), int(splits))
+
+
 def linear_status():
     s = C.c_int(0)
     _l.call("tcbnn_linear_status", C.byref(s))

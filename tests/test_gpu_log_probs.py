@@ -34,9 +34,9 @@ def order(logits, top):
     return torch.where(v == -math.inf, -1, i)[:, :top]
 
 
-def check(logits, targets, top, T=1.0):
+def check(logits, targets, top, T=1.0, answer=None):
     M, V = logits.shape
-    logp, entropy, ids, top_logp = ops.log_probs(logits, targets, top, T)
+    logp, entropy, ids, top_logp = answer or ops.log_probs(logits, targets, top, T)
     all_logp, want_h, E = definition(logits, T)
     steps = (V / 32 + 64) * 2.0 ** -24
     off_s = steps + 2.0 ** -21 + E * 2.0 ** -22
@@ -155,10 +155,9 @@ def test_nan_and_infinity_stay_in_their_row(cuda, dtype, V, value, masked):
         assert torch.equal(ids, order(clean, top))
     else:
         assert torch.equal(ids, order(clean, top)) and ids[2, 0] == V // 4 and ids[3, 0] == 0
-    again = ops.log_probs(x[keep], y[keep], top)
-    for a, b in zip((logp, entropy, ids, top_logp), again):
-        assert torch.equal(a[keep], b)
-    check(x[keep], y[keep], top)
+    # (not bit for bit what the rows alone give: a thread's share depends on where a row starts modulo 16 bytes, and with it
+    # the order of the sums)
+    check(x[keep], y[keep], top, answer=(logp[keep], entropy[keep], ids[keep], top_logp[keep]))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
