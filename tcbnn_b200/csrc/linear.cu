@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(256) k_repack(const uint16_t* src, long long l
     linear::repack(src, ld, rows, K, pitch, dst);
 }
 template <int TYPE, int NW, bool CLUSTER>
-__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32, NW == 1 ? 4 : 32 / NW) k_log_probs(scores::Args a) {
+__global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32, 32 / (NW == 1 ? 8 : NW)) k_log_probs(scores::Args a) {
     __shared__ scores::Shared<NW> shared[NW == 1 ? 8 : 1];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -209,13 +209,9 @@ int run_log_probs(const scores::Args& a, int sms, cudaStream_t st) {
         const cudaError_t e = launch_dependent(k_log_probs<TYPE, 1, false>, grid, 256, 0, st, a);
         return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
     }
-    if (batches < 16 || (batches < 32 && want < 8)) {
-        const cudaError_t e = launch_dependent(k_log_probs<TYPE, 4, false>, (unsigned)a.M, 128, 0, st, a);
-        return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
-    }
     unsigned ctas = 1;
     while (ctas < 8 && batches >= 32LL * ctas && want >= 32LL * ctas) ctas *= 2;
-    const cudaError_t e = ctas == 1 ? launch_dependent(k_log_probs<TYPE, 16, false>, (unsigned)a.M, 512, 0, st, a)
+    const cudaError_t e = ctas == 1 ? launch_dependent(k_log_probs<TYPE, 8, false>, (unsigned)a.M, 256, 0, st, a)
                                     : launch_dependent_cluster(k_log_probs<TYPE, 16, true>, (unsigned)a.M * ctas, ctas, 512, 0, st, a);
     return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
 }

@@ -4,14 +4,21 @@
 // -inf and entropy 0; one that holds NaN or +inf has NaN for both.  Alternatives are ordered by (logit, lowest token),
 // NaN taking no part.
 //
-// One pass over the row.  A thread keeps the maximum m, s = sum e^{(x-m)/T} and t = sum e^{(x-m)/T} (x-m) of what it has seen; a
-// batch of 64 bytes that raises m rescales both once.  The alternatives are kept by a threshold: of the threads' maxima of the
-// first batch the top-th largest (of the two best per warp) is a bound that at least `top` logits reach; what reaches it
-// goes to a list in shared memory (a few hundred of 100,000 logits in random order), which is sorted at the end, 32 keys
-// to a warp, and merged.  Where the list overflows -- logits in rising order, or more ties than it holds -- the row is read
-// again, the list cut to its best `top` as often as it fills.
+// One pass over the row.  With c = log2(e) / T and R = max(x) c rounded to a whole number, so that fma(x, c, -R) is rounded once, a
+// thread keeps the maximum m, R, s = sum 2^{xc - R} and t = sum 2^{xc - R} (xc - R) of what it has seen; a batch of 64 bytes that
+// raises R rescales both once.  R is at least -2^28, and logits below -1e30 (fp16: the lowest, -65504), masks among them, are
+// raised to that in front of the sums, two at a time in 16 bits: their terms are 0, and no product 0 * inf arises.  Rows for which
+// that does not hold -- |max(x) c| beyond 2^28, a maximum near -65504 in fp16, temperatures beyond 1e6 -- are summed again as they
+// are, from their maximum.
 //
-// A warp, 4 or 16 of them share a row, or the CTAs of a cluster, whose parts meet in the first one's shared memory.
+// Alternatives cost the pass nothing but the threads' maxima: at its end the top-th largest of them (of the best few per warp) is a
+// bound that at least `top` logits reach, hardly more when they come in random order; the few threads whose maximum reaches it have
+// their vectors read once more, by their whole warp, and what reaches the bound goes to a list in shared memory, which is
+// sorted, 32 keys to a warp, and merged.  (A threshold from the first 64 bytes of every thread, tested in the loop: 178 us against
+// 83 without alternatives at 4096 x 50001.)  Where the list overflows -- more ties than it holds -- the row is read again, the
+// list cut to its best `top` as often as it fills.
+//
+// A warp, 8 of them share a row, or the CTAs of a cluster, whose parts meet in the first one's shared memory.
 // Bound: HBM; 16-bit logits at 6.46 TB/s are 3.2e12 exponentials a second, 0.7 of what the units for them do.
 #pragma once
 #include "linear.cuh"
@@ -43,8 +50,9 @@ __device__ __forceinline__ float logit_of(unsigned long long key) {
 }
 __device__ __forceinline__ int token_of(unsigned long long key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
 
-// max m, sum e^{(x-m)/T} and sum e^{(x-m)/T} (x-m) of part of a row
-struct Sums { float m, s, t; };
+// maximum, R and the two sums of part of a row
+struct Sums { float m, ref, s, t; };
+constexpr float kLeastRef = -268435456.f;              // -2^28
 
 constexpr int kList1 = 256, kList = 2048;              // keys that a row's list holds: of a warp, of several
 constexpr uint32_t kAll = 0xffffffffu;
@@ -62,9 +70,38 @@ __device__ __forceinline__ uint4 load16(const void* p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+// what logits are raised to in front of the sums
+__host__ __device__ constexpr float lowest_of(int type) { return type == linear::FP16 ? -65504.f : -0x1.92p+99f; }      // (about -1e30)
 template <int TYPE>
 struct Element {
     static constexpr int kBytes = TYPE == linear::FP32 ? 4 : 2, kPer = 16 / kBytes;
+    static __device__ __forceinline__ uint32_t raise(uint32_t w) {           // (NaN stays)
+        uint32_t r;
+        if constexpr (TYPE == linear::FP32) asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xF1490000u));
+        else if constexpr (TYPE == linear::BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xF149F149u));
+        else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xFBFFFBFFu));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {      // (of NaN and a number the number)
+        uint32_t r;
+        if constexpr (TYPE == linear::FP32) asm("max.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else if constexpr (TYPE == linear::BF16) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float low(uint32_t w) {
+        if constexpr (TYPE == linear::FP32) return __uint_as_float(w);
+        else if constexpr (TYPE == linear::BF16) return __uint_as_float(w << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(w & 0xFFFFu)));
+    }
+    static __device__ __forceinline__ float high(uint32_t w) {
+        if constexpr (TYPE == linear::BF16) return __uint_as_float(w & 0xFFFF0000u);
+        else return __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+    }
+    static __device__ __forceinline__ float most(uint32_t w) {                // of a word
+        if constexpr (TYPE == linear::FP32) return __uint_as_float(w);
+        else return fmaxf(low(w), high(w));
+    }
     // element j of a vector
     static __device__ __forceinline__ float get(const uint4& v, int j) {
         if constexpr (TYPE == linear::FP32) {
@@ -104,8 +141,7 @@ struct Shared {
     unsigned long long list[NW == 1 ? kList1 : kList];
     unsigned long long best[NW == 1 ? 1 : 16][32];     // per warp; [0]: the row's
     Sums sums[16];
-    uint32_t maxima[32];
-    uint32_t threshold;
+    alignas(16) uint32_t maxima[32];
     int count;
     unsigned long long cut;                            // of the second reading: what does not exceed it is out
 };
@@ -115,7 +151,7 @@ __device__ __forceinline__ void meet() {
     else __syncthreads();
 }
 
-// the 32 best of the first `n` of the list, falling, in the lanes of warp 0 (and in s.best[0])
+// the 32 best of the first `n` of the list, falling, in the lanes of warp 0
 template <int NW>
 __device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n, int warp, int lane) {
     unsigned long long key = 0;
@@ -125,6 +161,7 @@ __device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n,
     }
     if constexpr (NW > 1) {
         const int lists = min(NW, (n + 31) >> 5);
+        if (lists <= 1) return key;
         s.best[warp][lane] = key;
         __syncthreads();
         for (int h = NW / 2; h; h /= 2) {
@@ -135,20 +172,50 @@ __device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n,
     return key;
 }
 
-__device__ __forceinline__ void reduce(Sums& q, float c) {                // over a warp
-    const float m = logit_of((unsigned long long)__reduce_max_sync(kAll, order_of(q.m)) << 32);
-    const uint32_t any = __reduce_max_sync(kAll, order_of(q.m));
-    if (any) {                                         // (0: nothing but -inf so far; sums are 0, or NaN)
-        const float d = q.m - m, f = ex2(d * c);
-        q.t = f == 0.f ? (q.s == q.s ? 0.f : q.s) : f * fmaf(q.s, d, q.t);
-        q.s = f == 0.f && q.s == q.s ? 0.f : f * q.s;
-        q.m = m;
-    }
+__device__ __forceinline__ float most_of_warp(float x) {                   // (-inf where nothing else is)
+    const uint32_t o = __reduce_max_sync(kAll, order_of(x));
+    return o ? logit_of((unsigned long long)o << 32) : -INFINITY;
+}
+__device__ __forceinline__ void reduce(Sums& q) {                         // over a warp
+    q.m = most_of_warp(q.m);
+    const float ref = most_of_warp(q.ref), d = q.ref - ref, f = ex2(d);
+    q.t = f * fmaf(q.s, d, q.t);
+    q.s = f * q.s;
+    q.ref = ref;
 #pragma unroll
     for (int h = 16; h; h /= 2) {
         q.s += __shfl_xor_sync(kAll, q.s, h);
         q.t += __shfl_xor_sync(kAll, q.t, h);
     }
+}
+template <int NW>
+__device__ __forceinline__ void reduce_row(Sums& q, Shared<NW>& s, int warp, int lane) {
+    reduce(q);
+    if constexpr (NW > 1) {
+        if (lane == 0) s.sums[warp] = q;
+        __syncthreads();
+        q = lane < NW ? s.sums[lane] : Sums{-INFINITY, kLeastRef, 0.f, 0.f};
+        reduce(q);
+    }
+}
+// The sums of a whole row as they are defined, from its maximum: R = 0 stands for mc.
+template <int TYPE, int NW>
+__device__ __forceinline__ void sum_again(const Args& a, Shared<NW>& s, const char* base, float c, int tid, int warp, int lane, Sums& q) {
+    constexpr int THREADS = NW * 32;
+    float m = -INFINITY;
+    for (int i = tid; i < a.V; i += THREADS) m = fmaxf(m, linear::load(base, i, TYPE));
+    q = Sums{m, 0.f, 0.f, 0.f};
+    meet<NW>();                                        // (s.sums is free)
+    reduce_row<NW>(q, s, warp, lane);
+    m = q.m;
+    q = Sums{m, 0.f, 0.f, 0.f};
+    for (int i = tid; i < a.V; i += THREADS) {
+        const float x = linear::load(base, i, TYPE), y = (x - m) * c, e = x == -INFINITY ? 0.f : ex2(y);
+        q.s += e;
+        q.t = fmaf(e, fmaxf(y, -3.0e38f), q.t);
+    }
+    meet<NW>();
+    reduce_row<NW>(q, s, warp, lane);
 }
 
 template <int TYPE, int NW, bool CLUSTER>
@@ -166,22 +233,23 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     const float c = a.inv_t * 1.44269504088896341f;    // log2 e / T
 
     if (tid == 0) { s.count = 0; s.cut = 0; }
-    Sums q{-INFINITY, 0.f, 0.f};
-    float thr = -INFINITY;
-    auto add_max = [&](float bm) {                     // a batch's maximum
+    Sums q{-INFINITY, kLeastRef, 0.f, 0.f};
+    auto raise_to = [&](float bm) {                    // a batch's maximum
         if (bm > q.m) {
-            if (q.m != -INFINITY) {
-                const float d = q.m - bm, f = ex2(d * c);
-                q.t = f == 0.f ? (q.t == q.t ? 0.f : q.t) : f * fmaf(q.s, d, q.t);
-                q.s *= f;
-            }
             q.m = bm;
+            const float ref = rintf(bm * c);
+            if (ref > q.ref) {
+                const float d = q.ref - ref, f = ex2(d);
+                q.t = f * fmaf(q.s, d, q.t);
+                q.s *= f;
+                q.ref = ref;
+            }
         }
     };
-    auto add_one = [&](float x, float m) {
-        const float d = x - m, e = ex2(d * c);
+    auto add = [&](float x) {
+        const float y = fmaf(x, c, -q.ref), e = ex2(y);
         q.s += e;
-        q.t = fmaf(e, fmaxf(d, -3.0e38f), q.t);
+        q.t = fmaf(e, y, q.t);
     };
     auto push = [&](float x, int token) {
         const unsigned long long key = key_of(x, token);
@@ -190,27 +258,20 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
             if (at < LIST) s.list[at] = key;
         }
     };
-    auto batch = [&](const uint4 (&v)[U], int i0) {    // vectors i0 + u * THREADS of the body
-        float bm = -INFINITY;
+    auto batch = [&](const uint4 (&v)[U]) {
+        uint32_t r[U][4], most = E::raise(v[0].x);
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            r[u][0] = E::raise(v[u].x); r[u][1] = E::raise(v[u].y); r[u][2] = E::raise(v[u].z); r[u][3] = E::raise(v[u].w);
+            most = E::larger(most, E::larger(E::larger(r[u][0], r[u][1]), E::larger(r[u][2], r[u][3])));
+        }
+        raise_to(E::most(most));
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int j = 0; j < PER; j++) bm = fmaxf(bm, E::get(v[u], j));
-        add_max(bm);
-        const float m = q.m == -INFINITY ? 0.f : q.m;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < PER; j++) add_one(E::get(v[u], j), m);
-        return bm;
-    };
-    auto push_batch = [&](const uint4 (&v)[U], int i0) {
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const float x = E::get(v[u], j);
-                if (x >= thr) push(x, head + (i0 + u * THREADS) * PER + j);
+            for (int j = 0; j < 4; j++) {
+                add(E::low(r[u][j]));
+                if constexpr (E::kPer == 8) add(E::high(r[u][j]));
             }
     };
     // (-inf: no part in anything)
@@ -223,81 +284,64 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     uint4 cur[U], next[U];
     int i0 = v0 + tid;
     load(cur, i0);
-    load(next, i0 + U * THREADS);
-    float bm = batch(cur, i0);
+    for (; i0 - lane < v1; i0 += U * THREADS) {        // (of the warp)
+        load(next, i0 + U * THREADS);
+        batch(cur);
+#pragma unroll
+        for (int u = 0; u < U; u++) cur[u] = next[u];
+    }
+    // the ends: a thread each
+    const float most = q.m;                            // of the vectors
+    int at = -1;
+    float end = -INFINITY;
+    if (first && tid < head) at = tid;
+    else if (last && tid >= 16 && tid - 16 < tail) at = head + vectors * PER + tid - 16;
+    if (at >= 0) {
+        end = linear::load(base, at, TYPE);
+        const float raised = end < lowest_of(TYPE) ? lowest_of(TYPE) : end;
+        raise_to(raised);
+        add(raised);
+    }
     if (a.top) {
-        uint32_t o = order_of(bm);
+        uint32_t o = most > lowest_of(TYPE) ? order_of(most) : 0u;
+        int more = 0;
         if constexpr (NW == 1) {
-            // the top-th largest of 32 maxima
-            int more = 0;
 #pragma unroll
             for (int i = 0; i < 32; i++) more += __shfl_sync(kAll, o, i) >= o;
-            o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
         } else {
-            constexpr int BEST = 32 / NW;              // per warp: 2 of 16, 8 of 4
+            constexpr int BEST = 32 / NW;              // per warp: 2 of 16, 4 of 8
             for (int i = 0; i < BEST; i++) {
-                const uint32_t most = __reduce_max_sync(kAll, o);
-                if (lane == 0) s.maxima[warp * BEST + i] = most;
-                if (lane == __ffs(__ballot_sync(kAll, o == most)) - 1) o = 0;
+                const uint32_t largest = __reduce_max_sync(kAll, o);
+                if (lane == 0) s.maxima[warp * BEST + i] = largest;
+                if (lane == __ffs(__ballot_sync(kAll, o == largest)) - 1) o = 0;
             }
             __syncthreads();
             o = s.maxima[lane];
-            int more = 0;
+            const uint4* all = reinterpret_cast<const uint4*>(s.maxima);
 #pragma unroll
-            for (int i = 0; i < 32; i++) more += s.maxima[i] >= o;
-            o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
-        }
-        thr = o ? logit_of((unsigned long long)o << 32) : -INFINITY;
-        if (NW == 1) __syncwarp();                     // (the count is 0)
-        if (bm >= thr) push_batch(cur, i0);
-    }
-    const int batches = (v1 - v0 + U * THREADS - 1) / (U * THREADS);     // (of every thread: the last ones may find nothing)
-    for (int b = 1; b < batches; b++) {
-        i0 += U * THREADS;
-#pragma unroll
-        for (int u = 0; u < U; u++) cur[u] = next[u];
-        load(next, i0 + U * THREADS);
-        bm = batch(cur, i0);
-        if (a.top && bm >= thr) push_batch(cur, i0);
-        if (NW > 1 && a.top && (b & 3) == 3) {
-            // a list that is half full gives a better bound, and room
-            __syncthreads();
-            const int n = s.count;
-            __syncthreads();
-            if (n > LIST / 2 && n <= LIST) {
-                const unsigned long long best = best_of_list<NW>(s, n, warp, lane);
-                if (warp == 0) {
-                    if (lane < a.top) s.list[lane] = best;
-                    if (lane == a.top - 1) s.cut = best;
-                    if (lane == 0) s.count = a.top;
-                }
-                __syncthreads();
-                thr = logit_of(s.cut);
+            for (int i = 0; i < 8; i++) {
+                const uint4 v = all[i];
+                more += (v.x >= o) + (v.y >= o) + (v.z >= o) + (v.w >= o);
             }
         }
-    }
-    // the ends: a thread each
-    {
-        int at = -1;
-        if (first && tid < head) at = tid;
-        else if (last && tid >= 16 && tid - 16 < tail) at = head + vectors * PER + tid - 16;
-        if (at >= 0) {
-            const float x = linear::load(base, at, TYPE);
-            add_max(x);
-            add_one(x, q.m == -INFINITY ? 0.f : q.m);
-            if (a.top && x >= thr) push(x, at);
+        o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
+        const float bound = o ? logit_of((unsigned long long)o << 32) : -INFINITY;
+        if (NW == 1) __syncwarp();                     // (the count is 0)
+        for (uint32_t hot = __ballot_sync(kAll, most >= bound); hot; hot &= hot - 1) {
+            const int of = tid - lane + __ffs(hot) - 1;                  // the thread
+            for (int i = v0 + of + lane * THREADS; i < v1; i += 32 * THREADS) {
+                const uint4 v = load16(body + (long long)i * 16);
+#pragma unroll
+                for (int j = 0; j < PER; j++) {
+                    const float x = E::get(v, j);
+                    if (x >= bound) push(x, head + i * PER + j);
+                }
+            }
         }
+        if (end >= bound && at >= 0) push(end, at);
     }
-    // sums of the row
-    reduce(q, c);
-    if constexpr (NW > 1) {
-        if (lane == 0) s.sums[warp] = q;
-        __syncthreads();
-        q = lane < NW ? s.sums[lane] : Sums{-INFINITY, 0.f, 0.f};
-        reduce(q, c);
-    } else {
-        __syncwarp();
-    }
+    reduce_row<NW>(q, s, warp, lane);
+    if constexpr (NW == 1) __syncwarp();
     // alternatives
     unsigned long long key = 0;
     if (a.top) {
@@ -353,14 +397,12 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
                 asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
                 return v;
             };
-            if (warp == 0) {
-                q = Sums{-INFINITY, 0.f, 0.f};
-                if ((uint32_t)lane < nctas) {
-                    const uint32_t at = peer(&s.sums[0], lane);
-                    q = Sums{ld(at), ld(at + 4), ld(at + 8)};
-                }
-                reduce(q, c);
+            q = Sums{-INFINITY, kLeastRef, 0.f, 0.f};
+            if ((uint32_t)lane < nctas) {
+                const uint32_t at = peer(&s.sums[0], lane);
+                q = Sums{ld(at), ld(at + 4), ld(at + 8), ld(at + 12)};
             }
+            reduce(q);
             if (a.top) {                               // warp w has the list of CTA w
                 if (warp > 0 && (uint32_t)warp < nctas)
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(peer(&s.best[0][lane], warp)) : "memory");
@@ -376,15 +418,19 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (!first) return;
     }
+    // terms of raised logits are 0, and what R was rounded by is at most 16
+    const bool right = a.inv_t >= 1e-6f && a.inv_t <= 1e6f && (q.m - lowest_of(TYPE)) * c > 150.f && fabsf(q.m * c) < -kLeastRef - 256.f;
+    if (!right) sum_again<TYPE, NW>(a, s, base, c, tid, warp, lane, q);
     if (warp == 0) {
-        const float lse = logf(q.s);
+        // ln sum e^{(x - m)/T}
+        const float lse = logf(q.s) - (right ? fmaf(q.m, c, -q.ref) * 0.693147180559945309f : 0.f);
         auto logp = [&](float x) { return x == -INFINITY ? (q.s == q.s ? -INFINITY : q.s) : fmaf(x - q.m, a.inv_t, -lse); };
         if (lane == 0) {
             if (a.logp) {
                 const long long y = a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
                 a.logp[r] = y < 0 ? 0.f : y >= a.V ? NAN : logp(linear::load(base, y, TYPE));
             }
-            if (a.entropy) a.entropy[r] = q.m == -INFINITY && q.s == 0.f ? 0.f : lse - q.t / q.s * a.inv_t;
+            if (a.entropy) a.entropy[r] = q.m == -INFINITY && q.s == 0.f ? 0.f : logf(q.s) - q.t / q.s * 0.693147180559945309f;
         }
         if (lane < a.top) {
             a.top_ids[r * a.top + lane] = key ? token_of(key) : -1;
