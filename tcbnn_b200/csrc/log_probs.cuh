@@ -142,6 +142,7 @@ struct Shared {
     unsigned long long best[NW == 1 ? 1 : 16][32];     // per warp; [0]: the row's
     Sums sums[16];
     alignas(16) uint32_t maxima[32];
+    unsigned char hot[16][32];                         // per warp: lanes whose maximum reaches the bound
     int count;
     unsigned long long cut;                            // of the second reading: what does not exceed it is out
 };
@@ -284,6 +285,12 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     uint4 cur[U], next[U];
     int i0 = v0 + tid;
     load(cur, i0);
+    long long target = -1;
+    float given = 0.f;
+    if (a.logp && tid == 0 && first) {                 // (under way while the row is read)
+        target = a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
+        if (target >= 0 && target < a.V) given = linear::load(base, target, TYPE);
+    }
     for (; i0 - lane < v1; i0 += U * THREADS) {        // (of the warp)
         load(next, i0 + U * THREADS);
         batch(cur);
@@ -327,15 +334,19 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
         const float bound = o ? logit_of((unsigned long long)o << 32) : -INFINITY;
         if (NW == 1) __syncwarp();                     // (the count is 0)
-        for (uint32_t hot = __ballot_sync(kAll, most >= bound); hot; hot &= hot - 1) {
-            const int of = tid - lane + __ffs(hot) - 1;                  // the thread
-            for (int i = v0 + of + lane * THREADS; i < v1; i += 32 * THREADS) {
-                const uint4 v = load16(body + (long long)i * 16);
+        // the vectors of the threads that reach it, over the lanes of their warp
+        const uint32_t hot = __ballot_sync(kAll, most >= bound);
+        if (most >= bound) s.hot[warp][__popc(hot & ((1u << lane) - 1))] = (unsigned char)lane;
+        __syncwarp();
+        const int each = (v1 - v0 - (tid - lane) + THREADS - 1) / THREADS, vs = each > 0 ? __popc(hot) * each : 0;      // (each: the first lane's)
+        for (int p = lane; p < vs; p += 32) {
+            const int h = p / each, i = v0 + tid - lane + s.hot[warp][h] + (p - h * each) * THREADS;
+            if (i >= v1) continue;
+            const uint4 v = load16(body + (long long)i * 16);
 #pragma unroll
-                for (int j = 0; j < PER; j++) {
-                    const float x = E::get(v, j);
-                    if (x >= bound) push(x, head + i * PER + j);
-                }
+            for (int j = 0; j < PER; j++) {
+                const float x = E::get(v, j);
+                if (x >= bound) push(x, head + i * PER + j);
             }
         }
         if (end >= bound && at >= 0) push(end, at);
@@ -415,6 +426,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
             }
         }
         __syncwarp();
+        // (nobody leaves before its part is read)
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (!first) return;
     }
@@ -426,10 +438,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         const float lse = logf(q.s) - (right ? fmaf(q.m, c, -q.ref) * 0.693147180559945309f : 0.f);
         auto logp = [&](float x) { return x == -INFINITY ? (q.s == q.s ? -INFINITY : q.s) : fmaf(x - q.m, a.inv_t, -lse); };
         if (lane == 0) {
-            if (a.logp) {
-                const long long y = a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
-                a.logp[r] = y < 0 ? 0.f : y >= a.V ? NAN : logp(linear::load(base, y, TYPE));
-            }
+            if (a.logp) a.logp[r] = target < 0 ? 0.f : target >= a.V ? NAN : logp(given);
             if (a.entropy) a.entropy[r] = q.m == -INFINITY && q.s == 0.f ? 0.f : logf(q.s) - q.t / q.s * 0.693147180559945309f;
         }
         if (lane < a.top) {
