@@ -95,7 +95,7 @@ int g_linear_cols = 0, g_linear_splits = 0;              // tcbnn_set_linear_pla
 
 // The plan with the least clocks.  A block of 64 of K costs a CTA its MMAs (cols / 2 each), its bytes from L2, or, with packed
 // weights, the expanders' time; a tile its set-up and what of the epilogue shows; a cluster its exchange.
-linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
+linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
     linear::Plan best = {};
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
@@ -131,6 +131,16 @@ linear::Plan plan_linear(int M, int N, int K, bool bits, int sms) {
         }
     }
     return best;
+}
+
+// (The last plans of this thread: the search takes a microsecond.)
+const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
+    struct Kept { int M, N, K, bits, sms, cols, splits; linear::Plan plan; };
+    static thread_local Kept kept[64];
+    Kept& k = kept[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 2246822519u ^ (unsigned)bits) >> 7 & 63];
+    if (k.M != M || k.N != N || k.K != K || k.bits != (int)bits || k.sms != sms || k.cols != g_linear_cols || k.splits != g_linear_splits)
+        k = Kept{M, N, K, (int)bits, sms, g_linear_cols, g_linear_splits, make_plan(M, N, K, bits, sms)};
+    return k.plan;
 }
 
 int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int width, int rows, long long pitch_bytes, int box_x, int box_y,
@@ -187,7 +197,7 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
         if (!bits && !rows_fit(a.W, a.ldw, a.N)) repack(&a.W, &a.ldw, a.N);
         if (launch_check(what)) return 1;
     }
-    const linear::Plan p = plan_linear(a.M, a.N, a.K, bits, sms);
+    const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, sms);
     const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap map_w, map_x;
     if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, p.cols, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
@@ -210,9 +220,11 @@ int run_log_probs(const scores::Args& a, int sms, cudaStream_t st) {
         return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
     }
     unsigned ctas = 1;
-    while (ctas < 8 && batches >= 32LL * ctas && want >= 32LL * ctas) ctas *= 2;
+    while (ctas < 8 && batches >= 16LL * ctas && 3 * want >= 32LL * ctas) ctas *= 2;
+    const bool wide = ctas == 8 && batches >= 128 && want >= 128;
     const cudaError_t e = ctas == 1 ? launch_dependent(k_log_probs<TYPE, 8, false>, (unsigned)a.M, 256, 0, st, a)
-                                    : launch_dependent_cluster(k_log_probs<TYPE, 16, true>, (unsigned)a.M * ctas, ctas, 512, 0, st, a);
+                        : wide      ? launch_dependent_cluster(k_log_probs<TYPE, 16, true>, (unsigned)a.M * ctas, ctas, 512, 0, st, a)
+                                    : launch_dependent_cluster(k_log_probs<TYPE, 8, true>, (unsigned)a.M * ctas, ctas, 256, 0, st, a);
     return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
 }
 

@@ -67,7 +67,7 @@ __device__ __forceinline__ uint32_t order_of(float x) { return (uint32_t)(key_of
 
 __device__ __forceinline__ uint4 load16(const void* p) {
     uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
 // what logits are raised to in front of the sums
@@ -140,7 +140,7 @@ template <int NW>
 struct Shared {
     unsigned long long list[NW == 1 ? kList1 : kList];
     unsigned long long best[NW == 1 ? 1 : 16][32];     // per warp; [0]: the row's
-    Sums sums[16];
+    Sums sums[17];                                     // per warp; [16]: of the CTA, for the cluster
     alignas(16) uint32_t maxima[32];
     unsigned char hot[16][32];                         // per warp: lanes whose maximum reaches the bound
     int count;
@@ -189,12 +189,15 @@ __device__ __forceinline__ void reduce(Sums& q) {                         // ove
         q.t += __shfl_xor_sync(kAll, q.t, h);
     }
 }
+// The sums of a warp's threads, into shared memory where several share the row; behind a barrier finish_row() gives the row's.
 template <int NW>
-__device__ __forceinline__ void reduce_row(Sums& q, Shared<NW>& s, int warp, int lane) {
+__device__ __forceinline__ void reduce_warps(Sums& q, Shared<NW>& s, int warp, int lane) {
     reduce(q);
+    if (NW > 1 && lane == 0) s.sums[warp] = q;
+}
+template <int NW>
+__device__ __forceinline__ void finish_row(Sums& q, Shared<NW>& s, int lane) {
     if constexpr (NW > 1) {
-        if (lane == 0) s.sums[warp] = q;
-        __syncthreads();
         q = lane < NW ? s.sums[lane] : Sums{-INFINITY, kLeastRef, 0.f, 0.f};
         reduce(q);
     }
@@ -207,7 +210,9 @@ __device__ __forceinline__ void sum_again(const Args& a, Shared<NW>& s, const ch
     for (int i = tid; i < a.V; i += THREADS) m = fmaxf(m, linear::load(base, i, TYPE));
     q = Sums{m, 0.f, 0.f, 0.f};
     meet<NW>();                                        // (s.sums is free)
-    reduce_row<NW>(q, s, warp, lane);
+    reduce_warps<NW>(q, s, warp, lane);
+    meet<NW>();
+    finish_row<NW>(q, s, lane);
     m = q.m;
     q = Sums{m, 0.f, 0.f, 0.f};
     for (int i = tid; i < a.V; i += THREADS) {
@@ -216,7 +221,9 @@ __device__ __forceinline__ void sum_again(const Args& a, Shared<NW>& s, const ch
         q.t = fmaf(e, fmaxf(y, -3.0e38f), q.t);
     }
     meet<NW>();
-    reduce_row<NW>(q, s, warp, lane);
+    reduce_warps<NW>(q, s, warp, lane);
+    meet<NW>();
+    finish_row<NW>(q, s, lane);
 }
 
 template <int TYPE, int NW, bool CLUSTER>
@@ -285,6 +292,12 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     uint4 cur[U], next[U];
     int i0 = v0 + tid;
     load(cur, i0);
+    // the ends: a thread each
+    int at = -1;
+    float end = -INFINITY;
+    if (first && tid < head) at = tid;
+    else if (last && tid >= 16 && tid - 16 < tail) at = head + vectors * PER + tid - 16;
+    if (at >= 0) end = linear::load(base, at, TYPE);
     long long target = -1;
     float given = 0.f;
     if (a.logp && tid == 0 && first) {                 // (under way while the row is read)
@@ -297,19 +310,14 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
 #pragma unroll
         for (int u = 0; u < U; u++) cur[u] = next[u];
     }
-    // the ends: a thread each
     const float most = q.m;                            // of the vectors
-    int at = -1;
-    float end = -INFINITY;
-    if (first && tid < head) at = tid;
-    else if (last && tid >= 16 && tid - 16 < tail) at = head + vectors * PER + tid - 16;
     if (at >= 0) {
-        end = linear::load(base, at, TYPE);
         const float raised = end < lowest_of(TYPE) ? lowest_of(TYPE) : end;
         raise_to(raised);
         add(raised);
     }
     if (a.top) {
+        reduce_warps<NW>(q, s, warp, lane);
         uint32_t o = most > lowest_of(TYPE) ? order_of(most) : 0u;
         int more = 0;
         if constexpr (NW == 1) {
@@ -351,8 +359,9 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         }
         if (end >= bound && at >= 0) push(end, at);
     }
-    reduce_row<NW>(q, s, warp, lane);
-    if constexpr (NW == 1) __syncwarp();
+    if (!a.top) reduce_warps<NW>(q, s, warp, lane);
+    meet<NW>();
+    finish_row<NW>(q, s, lane);
     // alternatives
     unsigned long long key = 0;
     if (a.top) {
@@ -393,7 +402,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         // the first CTA's first warp takes the others' parts
         if (warp == 0) {
             s.best[0][lane] = key;
-            if (lane == 0) s.sums[0] = q;
+            if (lane == 0) s.sums[16] = q;
         }
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -410,7 +419,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
             };
             q = Sums{-INFINITY, kLeastRef, 0.f, 0.f};
             if ((uint32_t)lane < nctas) {
-                const uint32_t at = peer(&s.sums[0], lane);
+                const uint32_t at = peer(&s.sums[16], lane);
                 q = Sums{ld(at), ld(at + 4), ld(at + 8), ld(at + 12)};
             }
             reduce(q);

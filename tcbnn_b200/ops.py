@@ -171,74 +171,84 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _TYPES = {torch.float32: _l.FP32, torch.float16: _l.FP16, torch.bfloat16: _l.BF16}
 
 
-def _rows(name, t, device, dtypes, width=None, rows=None):
+def _rows(name, t, device, dtype, width=None, rows=None):
     """Leading dimension of a 2-d operand on the current device whose rows are contiguous."""
+    if t.get_device() == device and t.dtype is dtype and t.dim() == 2:
+        r, w = t.shape
+        ld, inner = t.stride()
+        if (width is None or w == width) and (rows is None or r == rows) and (inner == 1 or w == 1):
+            if r <= 1:
+                return ld if ld > w else w
+            if ld >= w:
+                return ld
     if not t.is_cuda:
         raise _l.TcbnnError("tcbnn_b200 ops need CUDA tensors (no CPU path exists)")
-    if t.dim() != 2 or t.dtype not in dtypes or (width is not None and t.shape[1] != width) or (rows is not None and t.shape[0] != rows):
-        raise _l.TcbnnError(f"{name}: a tensor {[rows or 'rows', width or 'columns']} of {' or '.join(map(str, dtypes))} is wanted, "
-                            f"not {list(t.shape)} of {t.dtype}")
     if t.get_device() != device:
         raise _l.TcbnnError(f"{name} is on cuda:{t.get_device()}, the current device is cuda:{device}")
-    ld, inner = t.stride()
-    if inner != 1 and t.shape[1] != 1:
-        raise _l.TcbnnError(f"{name}: the elements of a row must be next to each other")
-    if t.shape[0] <= 1:
-        return max(ld, t.shape[1])
-    if ld < t.shape[1]:
-        raise _l.TcbnnError(f"{name}: rows overlap")
-    return ld
+    if t.dim() != 2 or t.dtype is not dtype or (width is not None and t.shape[1] != width) or (rows is not None and t.shape[0] != rows):
+        raise _l.TcbnnError(f"{name}: a tensor {[rows or 'rows', width or 'columns']} of {dtype} is wanted, not {list(t.shape)} of {t.dtype}")
+    raise _l.TcbnnError(f"{name}: rows must not overlap, nor the elements of a row lie apart (strides {t.stride()})")
 
 
 def _vector(name, t, device, dtypes, n):
-    """Pointer of a vector of n on the current device, None without one."""
-    if t is None:
-        return None
-    if not t.is_cuda or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous() or t.get_device() != device:
+    """Pointer of a vector of n on the current device."""
+    if t.get_device() != device or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
         raise _l.TcbnnError(f"{name}: a contiguous vector of {n} of {' or '.join(map(str, dtypes))} on cuda:{device} is wanted, "
                             f"not {list(t.shape)} of {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-_REAL16, _WORDS, _FP32 = (torch.bfloat16, torch.float16), (torch.int32,), (torch.float32,)
+_FP32 = (torch.float32,)
+_empty = torch.empty_strided          # (the cheapest of torch's ways to make a tensor)
 
 
 def _product(x, weight, scale, bias, activation, residual, out, out_dtype, workspace, bits):
-    device = _current_device()
-    xt = x.dtype
-    ldx = _rows("x", x, device, _REAL16)
+    device, xt = _current_device(), x.dtype
+    if xt is not torch.bfloat16 and xt is not torch.float16:
+        raise _l.TcbnnError(f"x is of torch.bfloat16 or torch.float16, not {xt}")
+    ldx = _rows("x", x, device, xt)
     M, K = x.shape
-    ldw = _rows("weight", weight, device, _WORDS if bits else (xt,), None if bits else K)
-    N = weight.shape[0]
-    if bits and weight.shape[1] * 32 < K:
-        raise _l.TcbnnError(f"weight: {weight.shape[1]} words do not hold {K} bits")
-    if activation not in ACTIVATIONS:
+    if bits:
+        ldw = _rows("weight", weight, device, torch.int32)
+        N, words = weight.shape
+        if words * 32 < K:
+            raise _l.TcbnnError(f"weight: {words} words do not hold {K} bits")
+    else:
+        ldw = _rows("weight", weight, device, xt, K)
+        N = weight.shape[0]
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise _l.TcbnnError(f"activation: one of {', '.join(ACTIVATIONS)} is wanted, not {activation!r}")
-    if out is not None:
-        out_dtype = out.dtype if out_dtype is None else out_dtype
-    elif out_dtype is None:
-        out_dtype = xt
-    if out_dtype is not xt and out_dtype is not torch.float32:
-        raise _l.TcbnnError(f"the result is of {xt} or torch.float32, not {out_dtype}")
-    ot = (out_dtype,)
+    ot = out_dtype if out_dtype is not None else xt if out is None else out.dtype
+    if ot is not xt and ot is not torch.float32:
+        raise _l.TcbnnError(f"the result is of {xt} or torch.float32, not {ot}")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=x.device)
-        ldo = N
+        out, ldo = _empty((M, N), (N, 1), dtype=ot, device=x.device), N
     else:
         ldo = _rows("out", out, device, ot, N, M)
-    ldr = 0 if residual is None else _rows("residual", residual, device, ot, N, M)
-    bias_p = _vector("bias", bias, device, (xt, torch.float32), N)
-    need = 0 if M == 0 else _l.bound("tcbnn_linear_workspace_bytes")(x.data_ptr(), None if bits else weight.data_ptr(), M, N, K, ldx, ldw)
-    if workspace is None and need:
-        workspace = torch.empty((need,), dtype=torch.uint8, device=x.device)
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    sizes = (M, N, K, ldx, ldw, ldr, ldo, _TYPES[xt], _TYPES[out_dtype], _TYPES[xt if bias is None else bias.dtype],
-             ACTIVATIONS[activation], ws, ws_bytes, _raw_stream(device))
+    bias_p, bt, res_p, ldr = None, xt, None, 0
+    if bias is not None:
+        bias_p, bt = _vector("bias", bias, device, (xt, torch.float32), N), bias.dtype
+    if residual is not None:
+        res_p, ldr = residual.data_ptr(), _rows("residual", residual, device, ot, N, M)
+    x_p, w_p, ws, ws_bytes = x.data_ptr(), weight.data_ptr(), None, 0
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif (x_p | 2 * ldx | (0 if bits else w_p | 2 * ldw)) & 15 and M:
+        # (rows that do not all start on 16 bytes)
+        ws_bytes = _l.bound("tcbnn_linear_workspace_bytes")(x_p, None if bits else w_p, M, N, K, ldx, ldw)
+        if ws_bytes:
+            workspace = _empty((ws_bytes,), (1,), dtype=torch.uint8, device=x.device)
+            ws = workspace.data_ptr()
     if bits:
-        _l.call("tcbnn_bit_linear", x.data_ptr(), weight.data_ptr(), _vector("scale", scale, device, _FP32, N), bias_p, _ptr(residual),
-                out.data_ptr(), *sizes)
+        rc = _l.bound("tcbnn_bit_linear")(x_p, w_p, None if scale is None else _vector("scale", scale, device, _FP32, N), bias_p, res_p,
+                                          out.data_ptr(), M, N, K, ldx, ldw, ldr, ldo, _TYPES[xt], _TYPES[ot], _TYPES[bt], act, ws, ws_bytes,
+                                          _raw_stream(device))
     else:
-        _l.call("tcbnn_linear", x.data_ptr(), weight.data_ptr(), bias_p, _ptr(residual), out.data_ptr(), *sizes)
+        rc = _l.bound("tcbnn_linear")(x_p, w_p, bias_p, res_p, out.data_ptr(), M, N, K, ldx, ldw, ldr, ldo, _TYPES[xt], _TYPES[ot], _TYPES[bt],
+                                      act, ws, ws_bytes, _raw_stream(device))
+    if rc:
+        _l.check(rc)
     return out
 
 
@@ -246,7 +256,7 @@ def linear_workspace(x, weight):
     """Scratch that linear() needs on these operands (bit_linear(): weight=None), or None; without one given it is
     allocated per call."""
     N, ldw = (1, 8) if weight is None else (weight.shape[0], weight.stride(0))
-    n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), _ptr(weight), x.shape[0], N, x.shape[1], max(x.stride(0), x.shape[1]), ldw)
+    n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), _ptr(weight), x.shape[0], N, x.shape[1], x.stride(0), ldw)
     return torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
 
 
@@ -280,19 +290,25 @@ def log_probs(logits, targets=None, top=0, temperature=1.0):
     distance apart) divided by `temperature` (tcbnn_log_probs).
     logp: of the given tokens targets [M] (int32 or int64), 0 where that is negative; None without targets.  top_ids (int64): the `top`
     likeliest tokens (at most 32), equal ones in rising order; -1 behind the last token whose logit is not -inf."""
-    device = _current_device()
-    ld = _rows("logits", logits, device, tuple(_TYPES))
+    device, code = _current_device(), _TYPES.get(logits.dtype)
+    if code is None:
+        raise _l.TcbnnError(f"logits are of torch.float32, torch.float16 or torch.bfloat16, not {logits.dtype}")
+    ld = _rows("logits", logits, device, logits.dtype)
     M, V = logits.shape
-    targets_p = _vector("targets", targets, device, (torch.int64, torch.int32), M)
     if not 0 <= top <= 32:
         raise _l.TcbnnError(f"top must be between 0 and 32, not {top}")
-    where = dict(dtype=torch.float32, device=logits.device)
-    logp = None if targets is None else torch.empty((M,), **where)
-    entropy, top_logp = torch.empty((M,), **where), torch.empty((M, top), **where)
-    top_ids = torch.empty((M, top), dtype=torch.int64, device=logits.device)
-    _l.call("tcbnn_log_probs", logits.data_ptr(), _TYPES[logits.dtype], M, V, ld, targets_p, 0 if targets is None else targets.element_size(),
-            temperature, top, _ptr(logp), entropy.data_ptr(), top_ids.data_ptr(), top_logp.data_ptr(), _raw_stream(device))
-    return logp, entropy, top_ids, top_logp
+    targets_p, target_bytes = None, 0
+    if targets is not None:
+        targets_p, target_bytes = _vector("targets", targets, device, (torch.int64, torch.int32), M), targets.element_size()
+    # (one allocation for what is fp32)
+    sizes = [0 if targets is None else M, M, M * top]
+    logp, entropy, top_logp = torch.unsafe_split_with_sizes(_empty((sum(sizes),), (1,), dtype=torch.float32, device=logits.device), sizes)
+    top_ids = _empty((M, top), (top or 1, 1), dtype=torch.int64, device=logits.device)
+    rc = _l.bound("tcbnn_log_probs")(logits.data_ptr(), code, M, V, ld, targets_p, target_bytes, temperature, top, logp.data_ptr(),
+                                     entropy.data_ptr(), top_ids.data_ptr(), top_logp.data_ptr(), _raw_stream(device))
+    if rc:
+        _l.check(rc)
+    return logp if targets is not None else None, entropy, top_ids, top_logp.view(M, top)
 
 
 def conv_desc(B, H, W, Cc, O, R, S, stride_h=1, stride_w=1, padding=True, pool=1):
