@@ -439,6 +439,9 @@ int tcbnn_set_linear_plan(int cols, int splits);
 int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, const void* targets, int target_bytes, float temperature,
                     int top, float* logp, float* entropy, int64_t* top_ids, float* top_logp, void* stream);
 
+/* Forces how a row of it is shared out: 1, 2, 4 or 8 warps (ctas 1), or clusters of 2, 4 or 8 CTAs of 8 warps; warps 0 = automatic.  Process-wide; for tests and measurements. */
+int tcbnn_set_log_probs_plan(int warps, int ctas);
+
 #ifdef __cplusplus
 }
 #endif

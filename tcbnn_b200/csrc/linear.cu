@@ -206,26 +206,35 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     return bits ? launch_linear<true>(a, p, sms, map_w, map_x, st) : launch_linear<false>(a, p, sms, map_w, map_x, st);
 }
 
-// How many warps share a row.  A warp's list holds 256 keys: it takes rows of up to eight batches of which no more than half as many are
-// expected to reach the bound, the top-th of 32 maxima over `per` logits each; 16 warps take rows that give every thread two batches, or
-// fewer where rows are few; beyond that the CTAs of a cluster, while every thread finds a batch.
+int g_scores_warps = 0, g_scores_ctas = 0;               // tcbnn_set_log_probs_plan: 0 = from the sizes
+
+// How many warps share a row.  As many as bring 32 to every SM, but no more than find a batch each; at least so many that a warp has
+// eight batches at most, that the vectors read once more (the share top / threads of the row) stay few, and, for more than 16
+// alternatives, that a bound from 32 maxima is not the least of them.  One warp, 2, 4, 8: 8192 x 1000 fp32 with 5 alternatives 13.4,
+// 21, 30, 53 us, with 32 71, 30, 39, 69; 2000 x 8000 bf16 21.8, 16.1, 15.1, 18.9; 500 x 4000 fp32 11.5, 8.4, 7.0, 6.1; 4096 x 50001 bf16
+// 168, 116, 91, 92.  Clusters of CTAs only where warps that find two batches are still wanted, as they cost 1 to 3 us: 256 x 50257 fp16
+// 21.2 us alone, 16.7 in pairs, 22.2 in fours; 300 x 32000 fp32 12.9, 17.7, 21; 1 x 131072 bf16 15.1, 10.8, 7.7, 6.5 in eights.
 template <int TYPE>
 int run_log_probs(const scores::Args& a, int sms, cudaStream_t st) {
     const int per = 4 * scores::Element<TYPE>::kPer;
-    const long long batches = (a.V + 32LL * per - 1) / (32 * per), want = 32LL * sms / a.M;
-    const double reach = a.top ? -log(1 - (a.top < 32 ? a.top : 31.5) / 32.0) / per * a.V : 0;
-    if ((batches < 4 || (batches <= 8 && want < 2)) && (reach <= 128 || a.V <= scores::kList1)) {
-        const unsigned grid = (unsigned)((a.M + 7LL) / 8);
-        const cudaError_t e = launch_dependent(k_log_probs<TYPE, 1, false>, grid, 256, 0, st, a);
+    const long long batches = (a.V + 32LL * per - 1) / (32 * per);
+    const double want = 32.0 * sms / a.M, most = (double)batches;
+    double need = want < most ? want : most;
+    if (need < most / 8) need = most / 8;
+    if (need < a.top * most / 64) need = a.top * most / 64;
+    if (a.top > 16 && need < 2) need = 2;
+    int warps = 1, ctas = 1;
+    while (warps < 8 && warps < need) warps *= 2;
+    while (warps == 8 && ctas < 8 && most >= 32.0 * ctas && want >= 16.0 * ctas) ctas *= 2;
+    if (g_scores_warps) { warps = g_scores_warps; ctas = g_scores_ctas; }
+    const auto go = [&](auto kernel) {
+        const unsigned grid = warps == 1 ? (unsigned)((a.M + 7LL) / 8) : (unsigned)a.M * ctas, threads = warps == 1 ? 256 : 32 * warps;
+        const cudaError_t e = launch_dependent_cluster(kernel, grid, ctas > 1 ? ctas : 0, threads, 0, st, a);
         return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
-    }
-    unsigned ctas = 1;
-    while (ctas < 8 && batches >= 16LL * ctas && 3 * want >= 32LL * ctas) ctas *= 2;
-    const bool wide = ctas == 8 && batches >= 128 && want >= 128;
-    const cudaError_t e = ctas == 1 ? launch_dependent(k_log_probs<TYPE, 8, false>, (unsigned)a.M, 256, 0, st, a)
-                        : wide      ? launch_dependent_cluster(k_log_probs<TYPE, 16, true>, (unsigned)a.M * ctas, ctas, 512, 0, st, a)
-                                    : launch_dependent_cluster(k_log_probs<TYPE, 8, true>, (unsigned)a.M * ctas, ctas, 256, 0, st, a);
-    return e != cudaSuccess ? fail("log_probs: %s", cudaGetErrorString(e)) : 0;
+    };
+    if (ctas > 1) return go(k_log_probs<TYPE, 8, true>);
+    return warps == 1 ? go(k_log_probs<TYPE, 1, false>) : warps == 2 ? go(k_log_probs<TYPE, 2, false>)
+         : warps == 4 ? go(k_log_probs<TYPE, 4, false>) : go(k_log_probs<TYPE, 8, false>);
 }
 
 }  // namespace
@@ -268,6 +277,14 @@ int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const
                      int activation, void* workspace, size_t workspace_bytes, void* stream) {
     const linear::Args a{x, W, scale, bias, residual, out, M, N, K, ldx, ldw, ldr, ldo, type, out_type, bias_type, activation};
     return run_linear("bit_linear", a, true, workspace, workspace_bytes, (cudaStream_t)stream);
+}
+
+int tcbnn_set_log_probs_plan(int warps, int ctas) {
+    const bool alone = ctas <= 1 && (warps == 1 || warps == 2 || warps == 4 || warps == 8), shared = (ctas == 2 || ctas == 4 || ctas == 8) && warps == 8;
+    if (warps && !alone && !shared) return fail("set_log_probs_plan: 1, 2, 4 or 8 warps, or 2, 4 or 8 CTAs of 8 warps");
+    g_scores_warps = warps;
+    g_scores_ctas = ctas < 1 ? 1 : ctas;
+    return 0;
 }
 
 int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, const void* targets, int target_bytes, float temperature,

@@ -54,7 +54,7 @@ __device__ __forceinline__ int token_of(unsigned long long key) { return (int)(0
 struct Sums { float m, ref, s, t; };
 constexpr float kLeastRef = -268435456.f;              // -2^28
 
-constexpr int kList1 = 256, kList = 2048;              // keys that a row's list holds: of a warp, of several
+__host__ __device__ constexpr int list_of(int warps) { return warps < 8 ? 256 * warps : 2048; }      // keys that a row's list holds
 constexpr uint32_t kAll = 0xffffffffu;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -127,6 +127,17 @@ __device__ __forceinline__ unsigned long long sort32(unsigned long long key) {
         for (int d = size / 2; d; d /= 2) exchange(key, d, ((lane & d) == 0) == ((lane & size) == 0));
     return key;
 }
+__device__ __forceinline__ uint32_t sort32(uint32_t v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int d = size / 2; d; d /= 2) {
+            const uint32_t o = __shfl_xor_sync(kAll, v, d);
+            v = ((lane & d) == 0) == ((lane & size) == 0) ? max(v, o) : min(v, o);
+        }
+    return v;
+}
 // the 32 best of two falling lists (`other` given in rising order)
 __device__ __forceinline__ unsigned long long merge32(unsigned long long key, unsigned long long other) {
     const int lane = threadIdx.x & 31;
@@ -138,11 +149,11 @@ __device__ __forceinline__ unsigned long long merge32(unsigned long long key, un
 
 template <int NW>
 struct Shared {
-    unsigned long long list[NW == 1 ? kList1 : kList];
-    unsigned long long best[NW == 1 ? 1 : 16][32];     // per warp; [0]: the row's
-    Sums sums[17];                                     // per warp; [16]: of the CTA, for the cluster
-    alignas(16) uint32_t maxima[32];
-    unsigned char hot[16][32];                         // per warp: lanes whose maximum reaches the bound
+    unsigned long long list[list_of(NW)];
+    unsigned long long best[NW][32];     // per warp; [0]: the row's
+    Sums sums[NW + 1];                                 // per warp; [NW]: of the CTA, for the cluster
+    uint32_t maxima[32];
+    unsigned char hot[NW][32];                         // per warp: lanes whose maximum reaches the bound
     int count;
     unsigned long long cut;                            // of the second reading: what does not exceed it is out
 };
@@ -155,6 +166,20 @@ __device__ __forceinline__ void meet() {
 // the 32 best of the first `n` of the list, falling, in the lanes of warp 0
 template <int NW>
 __device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n, int warp, int lane) {
+    if (n <= 32) {                                     // by counting: an eighth of the instructions of sorting six
+        if (warp == 0) {
+            const unsigned long long mine = lane < n ? s.list[lane] : 0ull;
+            int rank = 0;
+            for (int i = 0; i < n; i++) rank += s.list[i] > mine;
+            __syncwarp();
+            s.best[0][lane] = 0;
+            __syncwarp();
+            if (lane < n) s.best[0][rank] = mine;
+            __syncwarp();
+            return s.best[0][lane];
+        }
+        return 0ull;
+    }
     unsigned long long key = 0;
     for (int i = warp * 32; i < n; i += NW * 32) {
         const unsigned long long other = sort32(i + lane < n ? s.list[i + lane] : 0ull);
@@ -162,7 +187,6 @@ __device__ __forceinline__ unsigned long long best_of_list(Shared<NW>& s, int n,
     }
     if constexpr (NW > 1) {
         const int lists = min(NW, (n + 31) >> 5);
-        if (lists <= 1) return key;
         s.best[warp][lane] = key;
         __syncthreads();
         for (int h = NW / 2; h; h /= 2) {
@@ -177,9 +201,10 @@ __device__ __forceinline__ float most_of_warp(float x) {                   // (-
     const uint32_t o = __reduce_max_sync(kAll, order_of(x));
     return o ? logit_of((unsigned long long)o << 32) : -INFINITY;
 }
-__device__ __forceinline__ void reduce(Sums& q) {                         // over a warp
+__device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(rintf(m * c), kLeastRef); }
+__device__ __forceinline__ void reduce(Sums& q, float c) {                // over a warp
     q.m = most_of_warp(q.m);
-    const float ref = most_of_warp(q.ref), d = q.ref - ref, f = ex2(d);
+    const float ref = ref_of(q.m, c), d = q.ref - ref, f = ex2(d);
     q.t = f * fmaf(q.s, d, q.t);
     q.s = f * q.s;
     q.ref = ref;
@@ -191,15 +216,15 @@ __device__ __forceinline__ void reduce(Sums& q) {                         // ove
 }
 // The sums of a warp's threads, into shared memory where several share the row; behind a barrier finish_row() gives the row's.
 template <int NW>
-__device__ __forceinline__ void reduce_warps(Sums& q, Shared<NW>& s, int warp, int lane) {
-    reduce(q);
+__device__ __forceinline__ void reduce_warps(Sums& q, Shared<NW>& s, float c, int warp, int lane) {
+    reduce(q, c);
     if (NW > 1 && lane == 0) s.sums[warp] = q;
 }
 template <int NW>
-__device__ __forceinline__ void finish_row(Sums& q, Shared<NW>& s, int lane) {
+__device__ __forceinline__ void finish_row(Sums& q, Shared<NW>& s, float c, int lane) {
     if constexpr (NW > 1) {
         q = lane < NW ? s.sums[lane] : Sums{-INFINITY, kLeastRef, 0.f, 0.f};
-        reduce(q);
+        reduce(q, c);
     }
 }
 // The sums of a whole row as they are defined, from its maximum: R = 0 stands for mc.
@@ -210,26 +235,27 @@ __device__ __forceinline__ void sum_again(const Args& a, Shared<NW>& s, const ch
     for (int i = tid; i < a.V; i += THREADS) m = fmaxf(m, linear::load(base, i, TYPE));
     q = Sums{m, 0.f, 0.f, 0.f};
     meet<NW>();                                        // (s.sums is free)
-    reduce_warps<NW>(q, s, warp, lane);
+    reduce_warps<NW>(q, s, 0.f, warp, lane);
     meet<NW>();
-    finish_row<NW>(q, s, lane);
+    finish_row<NW>(q, s, 0.f, lane);
     m = q.m;
-    q = Sums{m, 0.f, 0.f, 0.f};
+    q = Sums{0.f, 0.f, 0.f, 0.f};
     for (int i = tid; i < a.V; i += THREADS) {
         const float x = linear::load(base, i, TYPE), y = (x - m) * c, e = x == -INFINITY ? 0.f : ex2(y);
         q.s += e;
         q.t = fmaf(e, fmaxf(y, -3.0e38f), q.t);
     }
     meet<NW>();
-    reduce_warps<NW>(q, s, warp, lane);
+    reduce_warps<NW>(q, s, 0.f, warp, lane);
     meet<NW>();
-    finish_row<NW>(q, s, lane);
+    finish_row<NW>(q, s, 0.f, lane);
+    q.m = m;
 }
 
 template <int TYPE, int NW, bool CLUSTER>
 __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, uint32_t rank, uint32_t nctas) {
     using E = Element<TYPE>;
-    constexpr int THREADS = NW * 32, PER = E::kPer, U = 4, LIST = NW == 1 ? kList1 : kList;
+    constexpr int THREADS = NW * 32, PER = E::kPer, U = 4, LIST = list_of(NW);
     const int tid = NW == 1 ? threadIdx.x & 31 : threadIdx.x, lane = tid & 31, warp = NW == 1 ? 0 : tid >> 5;
     const char* base = reinterpret_cast<const char*>(a.logits) + r * a.ld * E::kBytes;
     // elements in front of the first 16-byte boundary, vectors, elements behind them
@@ -245,7 +271,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     auto raise_to = [&](float bm) {                    // a batch's maximum
         if (bm > q.m) {
             q.m = bm;
-            const float ref = rintf(bm * c);
+            const float ref = ref_of(bm, c);
             if (ref > q.ref) {
                 const float d = q.ref - ref, f = ex2(d);
                 q.t = f * fmaf(q.s, d, q.t);
@@ -317,14 +343,10 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         add(raised);
     }
     if (a.top) {
-        reduce_warps<NW>(q, s, warp, lane);
+        reduce_warps<NW>(q, s, c, warp, lane);
         uint32_t o = most > lowest_of(TYPE) ? order_of(most) : 0u;
-        int more = 0;
-        if constexpr (NW == 1) {
-#pragma unroll
-            for (int i = 0; i < 32; i++) more += __shfl_sync(kAll, o, i) >= o;
-        } else {
-            constexpr int BEST = 32 / NW;              // per warp: 2 of 16, 4 of 8
+        if constexpr (NW > 1) {
+            constexpr int BEST = 32 / NW;              // per warp
             for (int i = 0; i < BEST; i++) {
                 const uint32_t largest = __reduce_max_sync(kAll, o);
                 if (lane == 0) s.maxima[warp * BEST + i] = largest;
@@ -332,14 +354,8 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
             }
             __syncthreads();
             o = s.maxima[lane];
-            const uint4* all = reinterpret_cast<const uint4*>(s.maxima);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const uint4 v = all[i];
-                more += (v.x >= o) + (v.y >= o) + (v.z >= o) + (v.w >= o);
-            }
         }
-        o = __reduce_max_sync(kAll, more >= a.top ? o : 0u);
+        o = __shfl_sync(kAll, sort32(o), a.top - 1);
         const float bound = o ? logit_of((unsigned long long)o << 32) : -INFINITY;
         if (NW == 1) __syncwarp();                     // (the count is 0)
         // the vectors of the threads that reach it, over the lanes of their warp
@@ -347,21 +363,26 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         if (most >= bound) s.hot[warp][__popc(hot & ((1u << lane) - 1))] = (unsigned char)lane;
         __syncwarp();
         const int each = (v1 - v0 - (tid - lane) + THREADS - 1) / THREADS, vs = each > 0 ? __popc(hot) * each : 0;      // (each: the first lane's)
+        const float per = 1.f / (float)each;
         for (int p = lane; p < vs; p += 32) {
-            const int h = p / each, i = v0 + tid - lane + s.hot[warp][h] + (p - h * each) * THREADS;
+            // (p / each: exact in fp32, as p + 1/2 is half of 1 / each off the next whole number at least, and p < 2^18; others divide)
+            const int h = vs <= 1 << 18 ? (int)(((float)p + 0.5f) * per) : p / each;
+            const int i = v0 + tid - lane + s.hot[warp][h] + (p - h * each) * THREADS;
             if (i >= v1) continue;
             const uint4 v = load16(body + (long long)i * 16);
+            uint32_t over = 0;
 #pragma unroll
-            for (int j = 0; j < PER; j++) {
-                const float x = E::get(v, j);
-                if (x >= bound) push(x, head + i * PER + j);
+            for (int j = 0; j < PER; j++) over |= E::get(v, j) >= bound ? 1u << j : 0u;
+            for (; over; over &= over - 1) {
+                const int e = head + i * PER + __ffs(over) - 1;
+                push(linear::load(base, e, TYPE), e);
             }
         }
         if (end >= bound && at >= 0) push(end, at);
     }
-    if (!a.top) reduce_warps<NW>(q, s, warp, lane);
+    if (!a.top) reduce_warps<NW>(q, s, c, warp, lane);
     meet<NW>();
-    finish_row<NW>(q, s, lane);
+    finish_row<NW>(q, s, c, lane);
     // alternatives
     unsigned long long key = 0;
     if (a.top) {
@@ -402,7 +423,7 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         // the first CTA's first warp takes the others' parts
         if (warp == 0) {
             s.best[0][lane] = key;
-            if (lane == 0) s.sums[16] = q;
+            if (lane == 0) s.sums[NW] = q;
         }
         __syncwarp();
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -419,10 +440,10 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
             };
             q = Sums{-INFINITY, kLeastRef, 0.f, 0.f};
             if ((uint32_t)lane < nctas) {
-                const uint32_t at = peer(&s.sums[16], lane);
+                const uint32_t at = peer(&s.sums[NW], lane);
                 q = Sums{ld(at), ld(at + 4), ld(at + 8), ld(at + 12)};
             }
-            reduce(q);
+            reduce(q, c);
             if (a.top) {                               // warp w has the list of CTA w
                 if (warp > 0 && (uint32_t)warp < nctas)
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(peer(&s.best[0][lane], warp)) : "memory");

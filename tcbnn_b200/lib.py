@@ -96,6 +96,7 @@ SIGNATURES = {
     "tcbnn_set_linear_plan": (_I, [_I, _I]),
     "tcbnn_linear": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
     "tcbnn_bit_linear": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
+    "tcbnn_set_log_probs_plan": (_I, [_I, _I]),
     "tcbnn_log_probs": (_I, [_P, _I, _I, _I, _LL, _P, _I, C.c_float, _I, _P, _P, _P, _P, _P]),
 }
 

@@ -285,6 +285,11 @@ def linear_status():
     return s.value
 
 
+def set_log_probs_plan(warps=0, ctas=1):
+    """Force the warps of a CTA and the CTAs that share a row of log_probs(); 0 = automatic."""
+    _l.call("tcbnn_set_log_probs_plan", int(warps), int(ctas))
+
+
 def log_probs(logits, targets=None, top=0, temperature=1.0):
     """(logp [M], entropy [M], top_ids [M][top], top_logp [M][top]) of logits [M][V] (fp32, fp16 or bf16, rows contiguous, any
     distance apart) divided by `temperature` (tcbnn_log_probs).

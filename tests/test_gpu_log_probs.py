@@ -123,6 +123,41 @@ def test_orders_ties_and_masks(cuda, dtype, V, kind):
     check(x, y, top)
 
 
+@pytest.mark.parametrize("warps,ctas", [(1, 1), (2, 1), (4, 1), (8, 1), (8, 2), (8, 4), (8, 8)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,V,top", [(3, 1, 1), (5, 9, 9), (9, 300, 32), (4, 2050, 5), (3, 30011, 32), (2, 100001, 20)])
+def test_every_way_to_share_a_row(cuda, warps, ctas, dtype, M, V, top):
+    """Random rows, one with more ties than any list holds, rising ones, masked ones; forced plans."""
+    x, y = rows(M, V, dtype, cuda, V + M)
+    n = torch.arange(V, device=cuda)
+    x[0] = 0.5
+    x[1] = (n.float() * (16.0 / V)).to(dtype)
+    x[-1, n % 5 != 2] = -math.inf
+    ops.set_log_probs_plan(warps, ctas)
+    try:
+        answer = ops.log_probs(x, y, top)
+    finally:
+        ops.set_log_probs_plan()
+    check(x, y, top, answer=answer)
+
+
+@pytest.mark.parametrize("value", [-1e4, -1e9, -1e20, -3e38])
+@pytest.mark.parametrize("warps,ctas", [(1, 1), (8, 1), (8, 4)])
+def test_masks_of_finite_values(cuda, value, warps, ctas):
+    """Masks by large negative numbers, in front of, between and behind what is allowed; and nothing else at all."""
+    V = 40000
+    for dtype in (torch.float32, torch.bfloat16) + ((torch.float16,) if value == -1e4 else ()):
+        x, y = rows(4, V, dtype, cuda, 3)
+        x[0, :30000], x[1, 10000:], x[2, ::2] = value, value, value
+        x[3] = value
+        ops.set_log_probs_plan(warps, ctas)
+        try:
+            for T in (1.0, 0.01, 50.0):
+                check(x, y, 9, T, answer=ops.log_probs(x, y, 9, T))
+        finally:
+            ops.set_log_probs_plan()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [1, 40, 3000, 70001])
 def test_rows_that_rule_out_everything(cuda, dtype, V):
