@@ -423,8 +423,8 @@ int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const
 /* Device-side status word of these kernels, read as tcbnn_gemm_status reads its own (synchronises; 0 = fine, 1 = a bounded wait
  * gave up and results since the last reading are not valid; reading a failure clears it). */
 int tcbnn_linear_status(int* status);
-/* Forces their tiles of `cols` tokens (16 to 256 in steps of 16) and the CTAs (1, 2, 4 or 8) that share K; 0 = automatic.
- * Process-wide; for tests and measurements. */
+/* Forces their tiles of `cols` tokens (16 to 256 in steps of 16) and the CTAs (1, 2, 4 or 8) that share K, or with splits = -2
+ * pairs of CTAs that share tiles of 256 outputs (cols in steps of 32); 0 = automatic.  Process-wide; for tests and measurements. */
 int tcbnn_set_linear_plan(int cols, int splits);
 /* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);

@@ -12,11 +12,11 @@ namespace {
 
 __device__ int g_linear_status;      // 1 after a bounded wait inside k_linear gave up
 
-template <bool BITS, bool CLUSTER>
+template <bool BITS, int FORM>
 __global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, 1)
 k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
-    linear::umma_cta<BITS, CLUSTER>(a, p, &map_w, &map_x, status, dyn_smem_linear);
+    linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
 }
 __global__ void __launch_bounds__(256) k_repack(const uint16_t* src, long long ld, int rows, int K, int pitch, uint16_t* dst) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product waits before it reads)
@@ -99,34 +99,37 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
     linear::Plan best = {};
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
-    for (int splits = 1; splits <= 8; splits *= 2) {
-        if (g_linear_splits && splits != g_linear_splits) continue;
+    for (int shape = 0; shape < 5; shape++) {
+        const bool pair = shape == 4;
+        const int splits = pair ? 1 : 1 << shape;
+        if (g_linear_splits && g_linear_splits != (pair ? -2 : splits)) continue;
         const int per = ((kblocks + splits - 1) / splits + unit - 1) / unit * unit;
         if (splits > 1 && (splits - 1) * per >= kblocks && !g_linear_splits) continue;       // (a CTA without work)
-        const int clusters = splits == 1 ? sms : splits == 2 ? sms / 2 : splits == 4 ? sms * 33 / 148 : sms * 15 / 148;
-        for (int cols = 16; cols <= linear::kMaxCols; cols += 16) {
+        const int teams = pair || splits == 2 ? sms / 2 : splits == 1 ? sms : splits == 4 ? sms * 33 / 148 : sms * 15 / 148;
+        for (int cols = pair ? 32 : 16; cols <= linear::kMaxCols; cols += pair ? 32 : 16) {
             linear::Plan p = {};
+            p.form = pair ? linear::PAIR : splits > 1 ? linear::SPLIT : linear::ALONE;
             p.cols = cols;
             p.splits = splits;
             p.tiles_m = (M + cols - 1) / cols;
-            p.tiles_n = (N + 127) / 128;
+            p.tiles_n = pair ? (N + 255) / 256 : (N + 127) / 128;
             const long long tiles = (long long)p.tiles_m * p.tiles_n;
             if (splits > 1 && tiles * splits > (1 << 20)) continue;
-            if (g_linear_cols ? cols != g_linear_cols : cols > 16 && cols >= M + 16) continue;
+            if (g_linear_cols ? cols != g_linear_cols : cols > 32 && cols >= M + 32) continue;
             p.kblocks = kblocks;
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
-            p.accumulators = tiles <= sms || (bits && cols > 192) ? 1 : 2;
+            p.accumulators = tiles <= teams || (bits && cols > 192) ? 1 : 2;
             p.ring = (512 - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
-            p.stages = (int)((226 * 1024 - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(cols, bits));
+            p.stages = (int)((226 * 1024 - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(p, bits));
             if (p.stages > linear::kMaxStages) p.stages = linear::kMaxStages;
-            if (linear::smem_bytes(p, bits) > 227 * 1024) continue;
-            const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + cols * 128.0;
+            while (linear::smem_bytes(p, bits) > 227 * 1024) p.stages--;
+            const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;
             double block = bytes / 72 > mma ? bytes / 72 : mma;
             if (bits && block < 130) block = 130;
-            const double finish = 400 + cols * 12.0, waves = (double)((tiles + clusters - 1) / clusters);
-            const double clocks = waves * (p.per * block + (p.accumulators == 1 ? finish : 200)) + finish + 2500 + (splits > 1 ? 2000 : 0);
+            const double finish = 400 + cols * 12.0, waves = (double)((tiles + teams - 1) / teams);
+            const double clocks = waves * (p.per * block + (p.accumulators == 1 ? finish : 200)) + finish + 2500 + (splits > 1 || pair ? 2000 : 0);
             if (clocks < least) { least = clocks; best = p; }
         }
     }
@@ -159,18 +162,21 @@ template <bool BITS>
 int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const CUtensorMap& map_w, const CUtensorMap& map_x, cudaStream_t st) {
     static bool done[64];
     if (configure_once(done, [] {
-            const cudaError_t e = cudaFuncSetAttribute(k_linear<BITS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-            return e != cudaSuccess ? e : cudaFuncSetAttribute(k_linear<BITS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            cudaError_t e = cudaFuncSetAttribute(k_linear<BITS, linear::ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(k_linear<BITS, linear::SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            return e != cudaSuccess ? e : cudaFuncSetAttribute(k_linear<BITS, linear::PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
         })) return 1;
     void* status = nullptr;
     CUDA_TRY(cudaGetSymbolAddress(&status, g_linear_status));
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const int threads = BITS ? linear::kThreadsBits : linear::kThreadsDense;
     const size_t smem = linear::smem_bytes(p, BITS);
-    const cudaError_t e = p.splits == 1 ? launch_dependent(k_linear<BITS, false>, (unsigned)(tiles < sms ? tiles : sms), threads, smem, st, a, p,
-                                                           (int*)status, map_w, map_x)
-                                        : launch_dependent_cluster(k_linear<BITS, true>, (unsigned)(tiles * p.splits), p.splits, threads, smem, st,
-                                                                   a, p, (int*)status, map_w, map_x);
+    const int team = p.form == linear::PAIR ? 2 : p.splits;
+    const long long teams = p.form == linear::SPLIT || tiles < sms / team ? tiles : sms / team;
+    auto kernel = p.form == linear::ALONE ? k_linear<BITS, linear::ALONE> : p.form == linear::SPLIT ? k_linear<BITS, linear::SPLIT>
+                                                                                                    : k_linear<BITS, linear::PAIR>;
+    const cudaError_t e = launch_dependent_cluster(kernel, (unsigned)(teams * team), team > 1 ? team : 0, threads, smem, st, a, p, (int*)status,
+                                                   map_w, map_x);
     if (e != cudaSuccess) return fail("linear: %s", cudaGetErrorString(e));
     return 0;
 }
@@ -200,7 +206,7 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, sms);
     const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap map_w, map_x;
-    if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, p.cols, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
+    if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, linear::own_cols(p), CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
     if (bits ? linear_map(&map_w, a.W, CU_TENSOR_MAP_DATA_TYPE_UINT32, (a.K + 31) / 32, a.N, a.ldw * 4, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B)
              : linear_map(&map_w, a.W, type, a.K, a.N, a.ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
     return bits ? launch_linear<true>(a, p, sms, map_w, map_x, st) : launch_linear<false>(a, p, sms, map_w, map_x, st);
@@ -254,8 +260,8 @@ int tcbnn_linear(const void* x, const void* W, const void* bias, const void* res
 }
 
 int tcbnn_set_linear_plan(int cols, int splits) {
-    if (cols < 0 || cols > linear::kMaxCols || cols % 16 || splits < 0 || splits > 8 || (splits & (splits - 1)))
-        return fail("set_linear_plan: cols is 0 or a multiple of 16 up to 256, splits is 0, 1, 2, 4 or 8");
+    if (cols < 0 || cols > linear::kMaxCols || cols % (splits == -2 ? 32 : 16) || (splits != -2 && (splits < 0 || splits > 8 || (splits & (splits - 1)))))
+        return fail("set_linear_plan: cols is 0 or a multiple of 16 up to 256, splits is 0, 1, 2, 4 or 8, or -2 (pairs; cols a multiple of 32)");
     g_linear_cols = cols;
     g_linear_splits = splits;
     return 0;

@@ -13,8 +13,10 @@
 // Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.  Packed weights cost a
 // sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port either.
 //
-// Where tiles of 128 x cols leave SMs idle, K is cut over a cluster's CTAs, whose sums meet in shared memory, in rank
-// order: the same result every time.
+// Where tiles of 128 x cols leave SMs idle, K is cut over a cluster's CTAs (SPLIT), whose sums meet in shared memory, in rank
+// order: the same result every time.  Where there are enough, pairs of SMs own tiles of 256 outputs (PAIR): each CTA holds its
+// 128 rows of W and half of the tokens' rows, the leader issues MMAs that read both (cta_group::2), so that rows of x
+// come from L2 and out of shared memory half as often.
 #pragma once
 #include "bconv_umma_pre.cuh"
 #include "linear.cuh"
@@ -26,16 +28,19 @@ constexpr int kThreadsDense = 11 * 32, kThreadsBits = 20 * 32;
 constexpr int kMaxCols = 256, kMaxStages = 12, kMaxRing = 8, kRawStages = 3;
 constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 rows of 64 elements, of 512 bits
 
+enum Form { ALONE = 0, SPLIT = 1, PAIR = 2 };
 struct Plan {
-    int cols, splits;                                  // tokens per tile (a multiple of 16), CTAs that share K
+    int form, cols, splits;                            // tokens per tile (a multiple of 16), CTAs that share K
     int tiles_m, tiles_n, band;                        // tiles of tokens and of outputs; token tiles worked on together
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
 };
-__host__ __device__ inline uint32_t stage_bytes(int cols, bool bits) { return (bits ? 0u : kWStage) + (uint32_t)cols * 128u; }
+// rows of x that a CTA holds of a tile
+__host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
+__host__ __device__ inline uint32_t stage_bytes(const Plan& p, bool bits) { return (bits ? 0u : kWStage) + (uint32_t)own_cols(p) * 128u; }
 // ring (where the cluster's sums go afterwards), raw bits, barriers; 1 KB for its alignment
 __host__ __device__ inline size_t ring_bytes(const Plan& p, bool bits) {
-    const size_t ring = (size_t)p.stages * stage_bytes(p.cols, bits), sums = p.splits > 1 ? (size_t)p.cols * 512 : 0;
+    const size_t ring = (size_t)p.stages * stage_bytes(p, bits), sums = p.splits > 1 ? (size_t)p.cols * 512 : 0;
     return ((ring > sums ? ring : sums) + 1023) & ~(size_t)1023;
 }
 __host__ __device__ inline size_t smem_bytes(const Plan& p, bool bits) {
@@ -46,37 +51,55 @@ __device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap* map,
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
 }
+// the same to the calling CTA of a pair, completing on the leader's barrier (no multicast)
+__device__ __forceinline__ void tensor_g2s_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t leader_bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar) : "memory");
+}
+// the commits of a pair arrive in both CTAs
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar) : "memory");
+    else
+        umma::mma_commit(bar);
+}
 // rows of 128 bytes, 128-byte swizzle, eight rows 1 KB apart from the next
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-// fp16 or bf16 operands, both K-major, fp32 sums, M = 128
-__device__ __forceinline__ uint32_t idesc_16(int type, int n) {
+// fp16 or bf16 operands, both K-major, fp32 sums
+__device__ __forceinline__ uint32_t idesc_16(int type, int m, int n) {
     const uint32_t f = type == BF16 ? 1u : 0u;
-    return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+    return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // Four MMAs over 64 elements of K: both operands 32 bytes (two 16-byte units of the descriptor) on each time, or A
 // eight columns of tensor memory.
-__device__ __forceinline__ void mma_64(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
-#define TCBNN_MMA(PRED)                                                                              \
+#define TCBNN_MMA_HEAD                                                                               \
+    "{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 da, db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t" \
+    "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
+#define TCBNN_MMA_SS(G, PRED)                                                                        \
     "mov.b64 da, {xa, %4};\n\tmov.b64 db, {xb, %4};\n\t"                                            \
-    "@pl tcgen05.mma.cta_group::1.kind::f16 [%1], da, db, %5, " PRED ";\n\tadd.u32 xa, xa, 2;\n\tadd.u32 xb, xb, 2;\n\t"
-    asm volatile("{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 da, db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t"
-                 "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
-                 TCBNN_MMA("pa") TCBNN_MMA("pt") TCBNN_MMA("pt") TCBNN_MMA("pt") "}"
-                 ::"r"(leader), "r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory");
-#undef TCBNN_MMA
-}
-__device__ __forceinline__ void mma_64_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
-#define TCBNN_MMA(PRED)                                                                              \
+    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%1], da, db, %5, " PRED ";\n\tadd.u32 xa, xa, 2;\n\tadd.u32 xb, xb, 2;\n\t"
+#define TCBNN_MMA_TS(G, PRED)                                                                        \
     "mov.b64 db, {xb, %4};\n\t"                                                                     \
-    "@pl tcgen05.mma.cta_group::1.kind::f16 [%1], [xa], db, %5, " PRED ";\n\tadd.u32 xa, xa, 8;\n\tadd.u32 xb, xb, 2;\n\t"
-    asm volatile("{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t"
-                 "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
-                 TCBNN_MMA("pa") TCBNN_MMA("pt") TCBNN_MMA("pt") TCBNN_MMA("pt") "}"
-                 ::"r"(leader), "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory");
-#undef TCBNN_MMA
+    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%1], [xa], db, %5, " PRED ";\n\tadd.u32 xa, xa, 8;\n\tadd.u32 xb, xb, 2;\n\t"
+#define TCBNN_MMA_RUN(OP, G)                                                                         \
+    asm volatile(TCBNN_MMA_HEAD OP(G, "pa") OP(G, "pt") OP(G, "pt") OP(G, "pt") "}"                  \
+                 ::"r"(leader), "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory")
+// a: descriptor (low half) of W in shared memory, or its address in tensor memory (TS)
+template <bool TS, bool PAIR>
+__device__ __forceinline__ void mma_64(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
+    if constexpr (TS && PAIR) TCBNN_MMA_RUN(TCBNN_MMA_TS, "2");
+    else if constexpr (TS) TCBNN_MMA_RUN(TCBNN_MMA_TS, "1");
+    else if constexpr (PAIR) TCBNN_MMA_RUN(TCBNN_MMA_SS, "2");
+    else TCBNN_MMA_RUN(TCBNN_MMA_SS, "1");
 }
+#undef TCBNN_MMA_RUN
+#undef TCBNN_MMA_TS
+#undef TCBNN_MMA_SS
+#undef TCBNN_MMA_HEAD
 // 32 signs as 16 pairs of +-1: register i holds elements 2i (low half) and 2i + 1, which are bits 31 - 2i and 30 - 2i.  `minus`:
 // -1 twice, whose signs a set bit turns.  The word is laid out once so that a shift brings both bits to their places.
 __device__ __forceinline__ void expand_signs(uint32_t w, uint32_t minus, uint32_t* r) {
@@ -147,15 +170,16 @@ struct Output {
     }
 };
 
-template <bool BITS, bool CLUSTER>
+template <bool BITS, int FORM>
 __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUtensorMap* map_w, const CUtensorMap* map_x, int* status,
                                          unsigned char* smem0) {
     using namespace umma;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem0) + 1023) & ~(uintptr_t)1023);
+    constexpr bool CLUSTER = FORM == SPLIT, PAIRED = FORM == PAIR;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t nctas = CLUSTER ? [] { uint32_t n; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }() : 1u;
-    const uint32_t rank = CLUSTER ? [] { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }() : 0u;
-    const uint32_t stage = stage_bytes(p.cols, BITS);
+    const uint32_t rank = CLUSTER || PAIRED ? [] { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }() : 0u;
+    const uint32_t stage = stage_bytes(p, BITS);
     unsigned char* sRaw = smem + ring_bytes(p, BITS);
     uint64_t* sBar = reinterpret_cast<uint64_t*>(sRaw + (BITS ? kRawStages * kRawStage : 0));
     // barriers: full[12] | empty[12] | ring full[8] | ring empty[8] | raw full[3] | raw empty[3] | sums full[2] | sums empty[2] | drain
@@ -172,9 +196,12 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     auto SEMPTY = [&](int b) { return bar0 + 8u * (48 + b); };
     const uint32_t DRAIN = bar0 + 8u * 50;
 
-    const int t_first = CLUSTER ? (int)(blockIdx.x / nctas) : (int)blockIdx.x, t_step = CLUSTER ? (int)(gridDim.x / nctas) : (int)gridDim.x;
+    // (a pair walks over the tiles together)
+    const int team = CLUSTER ? (int)nctas : PAIRED ? 2 : 1;
+    const int t_first = (int)blockIdx.x / team, t_step = (int)gridDim.x / team;
     const int ntiles = p.tiles_m * p.tiles_n;
-    const int kb0 = (int)rank * p.per, nkb = max(0, min(p.per, p.kblocks - kb0));     // this CTA's blocks of K
+    const int kb0 = CLUSTER ? (int)rank * p.per : 0, nkb = max(0, min(p.per, p.kblocks - kb0));     // this CTA's blocks of K
+    const int n_of = PAIRED ? 256 : 128, n_own = PAIRED ? (int)rank * 128 : 0, own = own_cols(p);
     // bands of token tiles, in a band the tokens fastest: what runs together shares rows of both operands
     auto tile = [&](int t, int& tm, int& tn) {
         const int full = p.band * p.tiles_n, b = t / full, r = t - b * full, w = min(p.band, p.tiles_m - b * p.band);
@@ -184,22 +211,30 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
 
     if (tid == 0) {
         for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
-        for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), 4); mbar_init(REMPTY(s), 1); }
+        for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), PAIRED ? 8 : 4); mbar_init(REMPTY(s), 1); }
         for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 8); }
-        for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), 8); }
+        for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), PAIRED ? 16 : 8); }
         mbar_init(DRAIN, 1);
         *sAbort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 10) tmem_alloc(smem_u32(sTmem), 512);
+    if (warp == 10) {
+        if constexpr (PAIRED) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(smem_u32(sTmem), 512);
+        }
+    }
     fence_proxy_async();
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIRED) cluster_sync();                // the partner's barriers and tensor memory are set up as well
     tc_fence_after();
     const uint32_t tmem = *sTmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (not before the allocation: see bconv_umma_pre.cuh)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const WsWait wait{sAbort, status};
+    const typename std::conditional<PAIRED, PairWait, WsWait>::type wait{sAbort, status};
     const uint32_t ring_col = (uint32_t)(p.accumulators * p.cols);
 
     if (warp == 8 || warp == 9) {
@@ -218,32 +253,43 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                     if (!ok) break;
                     if (BITS && isw) {
                         mbar_expect_tx(RAWFULL(s), kRawStage);
-                        tensor_g2s(smem_u32(sRaw) + s * kRawStage, map_w, (kb0 + kb) * 2, tn * 128, RAWFULL(s));
+                        tensor_g2s(smem_u32(sRaw) + s * kRawStage, map_w, (kb0 + kb) * 2, tn * n_of + n_own, RAWFULL(s));
                     } else {
-                        const uint32_t bytes = isw ? kWStage : (uint32_t)p.cols * 128u;
-                        mbar_expect_tx(FULL(s), bytes);
-                        tensor_g2s(smem_u32(smem) + s * stage + (isw || BITS ? 0u : kWStage), isw ? map_w : map_x, (kb0 + kb) * 64,
-                                   isw ? tn * 128 : tm * p.cols, FULL(s));
+                        const uint32_t bytes = isw ? kWStage : (uint32_t)own * 128u, dst = smem_u32(smem) + s * stage + (isw || BITS ? 0u : kWStage);
+                        const int y = isw ? tn * n_of + n_own : tm * p.cols + (PAIRED ? (int)rank * own : 0);
+                        if constexpr (PAIRED) {          // (rows past the end arrive as zeros, and count)
+                            if (rank == 0) mbar_expect_tx(FULL(s), 2 * bytes);
+                            tensor_g2s_pair(dst, isw ? map_w : map_x, (kb0 + kb) * 64, y, leader_address(FULL(s)));
+                        } else {
+                            mbar_expect_tx(FULL(s), bytes);
+                            tensor_g2s(dst, isw ? map_w : map_x, (kb0 + kb) * 64, y, FULL(s));
+                        }
                     }
                     issued++;
                     if (++s == slots) { s = 0; ph ^= 1; }
                 }
             }
             if (!ok) {
-                // giving up: wait (bounded) for the copies still in flight before the CTA exits
+                // giving up: wait (bounded) for the copies still in flight before the CTA exits (the second CTA of a pair,
+                // whose copies complete on the other's barriers, lets the time of any copy pass)
+                const bool here = !PAIRED || rank == 0 || (BITS && isw);
                 for (int s2 = 0; s2 < slots; s2++) {
                     const bool this_pass = s2 < s;
                     if (!this_pass && issued < slots) continue;
-                    for (int i = 0; i < (1 << 20); i++)
-                        if (mbar_try_wait(BITS && isw ? RAWFULL(s2) : FULL(s2), this_pass ? ph : ph ^ 1)) break;
+                    for (int i = 0; i < (1 << 16); i++) {
+                        if (here && mbar_try_wait(BITS && isw ? RAWFULL(s2) : FULL(s2), this_pass ? ph : ph ^ 1)) break;
+                        __nanosleep(20);
+                    }
                 }
             }
         }
         __syncwarp();
+    } else if (PAIRED && warp == 10 && rank == 1) {
+        __syncwarp();                                    // (the leader issues for both)
     } else if (warp == 10) {
         // =============================== MMA issuer =========================================
         const uint32_t leader = elect_one() ? 1u : 0u;
-        const uint32_t idesc = idesc_16(a.type, p.cols);
+        const uint32_t idesc = idesc_16(a.type, PAIRED ? 256 : 128, p.cols);
         const uint64_t desc0 = swizzled_desc(smem_u32(smem));
         const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
         int s = 0, r = 0, b = 0;
@@ -260,12 +306,11 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t lo = lo0 + (s * stage >> 4);
-                    if constexpr (BITS) mma_64_ts(leader, d, tmem + ring_col + r * 32, lo, hi, idesc, kb > 0);
-                    else mma_64(leader, d, lo, lo + (kWStage >> 4), hi, idesc, kb > 0);
+                    mma_64<BITS, PAIRED>(leader, d, BITS ? tmem + ring_col + r * 32 : lo, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > 0);
                     if (leader) {
-                        mma_commit(EMPTY(s));
-                        if (BITS) mma_commit(REMPTY(r));
-                        if (kb + 1 == nkb) mma_commit(SFULL(b));
+                        commit<PAIRED>(EMPTY(s));
+                        if (BITS) commit<PAIRED>(REMPTY(r));
+                        if (kb + 1 == nkb) commit<PAIRED>(SFULL(b));
                     }
                     __syncwarp();
                     if (++s == p.stages) { s = 0; ph ^= 1; }
@@ -275,9 +320,10 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             }
         if (!ok && leader) {
             // giving up: the MMAs already issued must have finished before tensor memory is freed
-            mma_commit(DRAIN);
+            if constexpr (PAIRED) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(DRAIN) : "memory");
+            else mma_commit(DRAIN);
             for (int i = 0; i < (1 << 20); i++)
-                if (mbar_try_wait(DRAIN, 0)) break;
+                if (PAIRED ? mbar_test_cluster(DRAIN, 0) : mbar_try_wait(DRAIN, 0)) break;
         }
         __syncwarp();
     } else if (BITS && warp >= 12) {
@@ -312,7 +358,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(RFULL(r));
+                        if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(RFULL(r)); else mbar_arrive(RFULL(r)); }
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(RAWEMPTY(raw));
@@ -330,7 +376,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         for (int t = t_first; t < ntiles && ok; t += t_step) {
             int tm, tn;
             tile(t, tm, tn);
-            const Output out(a, tn * 128 + quad * 32 + lane);
+            const Output out(a, tn * n_of + n_own + quad * 32 + lane);
             if (nkb > 0) ok = wait.relaxed(SFULL(b), bph);
             if (!ok) break;
             tc_fence_after();
@@ -356,7 +402,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             }
             tc_fence_before();                           // this warp is done with the sums
             __syncwarp();
-            if (lane == 0) mbar_arrive(SEMPTY(b));
+            if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(SEMPTY(b)); else mbar_arrive(SEMPTY(b)); }
             if (++b == p.accumulators) { b = 0; bph ^= 1; }
         }
     }
@@ -387,7 +433,12 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         cluster_sync();                                  // nobody reads this CTA's sums any more
     }
     __syncthreads();
-    if (warp == 10) tmem_dealloc(tmem, 512);
+    if constexpr (PAIRED) {
+        cluster_sync();                                  // nothing of the partner's reaches into this CTA any more
+        if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    } else if (warp == 10) {
+        tmem_dealloc(tmem, 512);
+    }
 }
 
 // Rows of K elements of 16 bits, any distance apart, to rows of `pitch` elements

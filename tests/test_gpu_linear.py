@@ -86,6 +86,23 @@ def test_whole_numbers_come_out_exactly(cuda, bits, M, N, K):
 
 
 @pytest.mark.parametrize("bits", [False, True])
+@pytest.mark.parametrize("cols,splits", [(16, 1), (48, 1), (144, 1), (192, 1), (208, 1), (256, 1), (16, 2), (96, 2), (32, 4), (240, 4), (16, 8), (128, 8), (256, 8),
+                                         (32, -2), (96, -2), (192, -2), (224, -2), (256, -2)])
+@pytest.mark.parametrize("M,N,K", [(1, 128, 64), (300, 700, 1000), (530, 1300, 520), (40, 129, 8200), (2000, 5000, 72), (5000, 1500, 640)])
+def test_every_plan(cuda, bits, cols, splits, M, N, K):
+    """Forced tiles: one and several per CTA, more splits than there is K for, pairs with half of their outputs or tokens missing."""
+    x, w, scale, sums = case(bits, M, N, K, BF16, cuda)
+    bias, res = whole(gen(M), (N,), 50, FP32, cuda), whole(gen(N), (M, N), 50, FP32, cuda)
+    ops.set_linear_plan(cols, splits)
+    try:
+        got = product(bits, x, w, scale, bias, "relu", res, out_dtype=FP32)
+        assert ops.linear_status() == 0
+    finally:
+        ops.set_linear_plan()
+    assert torch.equal(got.double(), (sums + bias.double()).clamp(min=0) + res.double())
+
+
+@pytest.mark.parametrize("bits", [False, True])
 @pytest.mark.parametrize("name", ["relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("dtype,out", [(BF16, BF16), (FP16, FP16), (BF16, FP32), (FP16, FP32)])
 def test_activations(cuda, bits, name, dtype, out):
@@ -226,6 +243,7 @@ def test_on_other_streams_and_in_graphs(cuda, bits, M, N, K):
             g.replay()
     torch.cuda.synchronize()
     assert torch.equal(graphs[0][2], 2 * want) and torch.equal(graphs[1][2], want)
+    assert ops.linear_status() == 0
 
 
 @pytest.mark.parametrize("bits", [False, True])
