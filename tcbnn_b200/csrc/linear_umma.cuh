@@ -56,15 +56,6 @@ __device__ __forceinline__ void tensor_g2s_pair(uint32_t dst, const CUtensorMap*
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                  ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(leader_bar) : "memory");
 }
-// the commits of a pair arrive in both CTAs
-template <bool PAIR>
-__device__ __forceinline__ void commit(uint32_t bar) {
-    if constexpr (PAIR)
-        asm volatile("{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
-                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}" ::"r"(bar) : "memory");
-    else
-        umma::mma_commit(bar);
-}
 // rows of 128 bytes, 128-byte swizzle, eight rows 1 KB apart from the next
 __device__ __forceinline__ uint64_t swizzled_desc(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFFu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
@@ -75,31 +66,47 @@ __device__ __forceinline__ uint32_t idesc_16(int type, int m, int n) {
     return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 // Four MMAs over 64 elements of K: both operands 32 bytes (two 16-byte units of the descriptor) on each time, or A
-// eight columns of tensor memory.
-#define TCBNN_MMA_HEAD                                                                               \
-    "{\n\t.reg .pred pa, pt, pl;\n\t.reg .b64 da, db;\n\t.reg .b32 xa, xb;\n\tsetp.ne.b32 pa, %6, 0;\n\t" \
-    "setp.ne.b32 pl, %0, 0;\n\tsetp.eq.b32 pt, %0, %0;\n\tmov.u32 xa, %2;\n\tmov.u32 xb, %3;\n\t"
+// eight columns of tensor memory.  The commits of a pair arrive in both CTAs.
+// As one block with the tests of the barriers of the next stage (and, TS, of the next W operand) in front and their answers read
+// behind: a test takes 150-200 clocks to return while the MMAs keep the shared-memory port busy, and the tensor pipe queues no more
+// than two or three instructions.  Then the commits of the stage, of the operand and (bar_c != 0) of the sums.
+// a: descriptor (low half) of W in shared memory, or its address in tensor memory (TS).  Bit 0 / 1 of the result: phase par0 / par1
+// of bar0 / bar1 is complete.
 #define TCBNN_MMA_SS(G, PRED)                                                                        \
-    "mov.b64 da, {xa, %4};\n\tmov.b64 db, {xb, %4};\n\t"                                            \
-    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%1], da, db, %5, " PRED ";\n\tadd.u32 xa, xa, 2;\n\tadd.u32 xb, xb, 2;\n\t"
+    "mov.b64 da, {xa, %5};\n\tmov.b64 db, {xb, %5};\n\t"                                            \
+    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%2], da, db, %6, " PRED ";\n\tadd.u32 xa, xa, 2;\n\tadd.u32 xb, xb, 2;\n\t"
 #define TCBNN_MMA_TS(G, PRED)                                                                        \
-    "mov.b64 db, {xb, %4};\n\t"                                                                     \
-    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%1], [xa], db, %5, " PRED ";\n\tadd.u32 xa, xa, 8;\n\tadd.u32 xb, xb, 2;\n\t"
-#define TCBNN_MMA_RUN(OP, G)                                                                         \
-    asm volatile(TCBNN_MMA_HEAD OP(G, "pa") OP(G, "pt") OP(G, "pt") OP(G, "pt") "}"                  \
-                 ::"r"(leader), "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc) : "memory")
-// a: descriptor (low half) of W in shared memory, or its address in tensor memory (TS)
+    "mov.b64 db, {xb, %5};\n\t"                                                                     \
+    "@pl tcgen05.mma.cta_group::" G ".kind::f16 [%2], [xa], db, %6, " PRED ";\n\tadd.u32 xa, xa, 8;\n\tadd.u32 xb, xb, 2;\n\t"
+#define TCBNN_MMA_RUN(OP, SECOND, G, Q, W, B)                                                        \
+    asm volatile("{\n\t.reg .pred p0, p1, pa, pt, pl, pc, ps;\n\t.reg .b64 da, db;\n\t.reg .b32 xa, xb, r1;\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t" \
+                 "mbarrier.test_wait.parity" Q ".shared::cta.b64 p0, [%8], %9;\n\t"                  \
+                 "setp.ne.b32 p1, %1, %1;\n\t" SECOND("mbarrier.test_wait.parity" Q ".shared::cta.b64 p1, [%10], %11;\n\t") \
+                 "setp.ne.b32 pa, %7, 0;\n\tsetp.ne.b32 pl, %1, 0;\n\tsetp.eq.b32 pt, %1, %1;\n\tsetp.ne.and.b32 pc, %14, 0, pl;\n\t" \
+                 "mov.u32 xa, %3;\n\tmov.u32 xb, %4;\n\t" OP(G, "pa") OP(G, "pt") OP(G, "pt") OP(G, "pt") \
+                 "@pl tcgen05.commit.cta_group::" G ".mbarrier::arrive::one.shared::cluster" W ".b64 [%12]" B ";\n\t" \
+                 SECOND("@pl tcgen05.commit.cta_group::" G ".mbarrier::arrive::one.shared::cluster" W ".b64 [%13]" B ";\n\t") \
+                 "@pc tcgen05.commit.cta_group::" G ".mbarrier::arrive::one.shared::cluster" W ".b64 [%14]" B ";\n\t" \
+                 "selp.u32 %0, 1, 0, p0;\n\tselp.u32 r1, 2, 0, p1;\n\tor.b32 %0, %0, r1;\n\t}"      \
+                 : "=&r"(ok) : "r"(leader), "r"(d), "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"(acc), "r"(bar0), "r"(par0), "r"(bar1), \
+                   "r"(par1), "r"(bar_e), "r"(bar_r), "r"(bar_c) : "memory")
+#define TCBNN_YES(X) X
+#define TCBNN_NO(X) ""
 template <bool TS, bool PAIR>
-__device__ __forceinline__ void mma_64(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc) {
-    if constexpr (TS && PAIR) TCBNN_MMA_RUN(TCBNN_MMA_TS, "2");
-    else if constexpr (TS) TCBNN_MMA_RUN(TCBNN_MMA_TS, "1");
-    else if constexpr (PAIR) TCBNN_MMA_RUN(TCBNN_MMA_SS, "2");
-    else TCBNN_MMA_RUN(TCBNN_MMA_SS, "1");
+__device__ __forceinline__ uint32_t mma_64(uint32_t leader, uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t acc,
+                                           uint32_t bar0, uint32_t par0, uint32_t bar1, uint32_t par1, uint32_t bar_e, uint32_t bar_r, uint32_t bar_c) {
+    uint32_t ok;
+    if constexpr (TS && PAIR) TCBNN_MMA_RUN(TCBNN_MMA_TS, TCBNN_YES, "2", ".acquire.cluster", ".multicast::cluster", ", both");
+    else if constexpr (TS) TCBNN_MMA_RUN(TCBNN_MMA_TS, TCBNN_YES, "1", "", "", "");
+    else if constexpr (PAIR) TCBNN_MMA_RUN(TCBNN_MMA_SS, TCBNN_NO, "2", ".acquire.cluster", ".multicast::cluster", ", both");
+    else TCBNN_MMA_RUN(TCBNN_MMA_SS, TCBNN_NO, "1", "", "", "");
+    return ok;
 }
+#undef TCBNN_YES
+#undef TCBNN_NO
 #undef TCBNN_MMA_RUN
 #undef TCBNN_MMA_TS
 #undef TCBNN_MMA_SS
-#undef TCBNN_MMA_HEAD
 // 32 signs as 16 pairs of +-1: register i holds elements 2i (low half) and 2i + 1, which are bits 31 - 2i and 30 - 2i.  `minus`:
 // -1 twice, whose signs a set bit turns.  The word is laid out once so that a shift brings both bits to their places.
 __device__ __forceinline__ void expand_signs(uint32_t w, uint32_t minus, uint32_t* r) {
@@ -293,7 +300,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         const uint64_t desc0 = swizzled_desc(smem_u32(smem));
         const uint32_t hi = (uint32_t)(desc0 >> 32), lo0 = (uint32_t)desc0;
         int s = 0, r = 0, b = 0;
-        uint32_t ph = 0, rph = 0, bph = 0;
+        uint32_t ph = 0, rph = 0, bph = 0, ready = 0;
         bool ok = true;
         if (nkb > 0)
             for (int t = t_first; t < ntiles && ok; t += t_step) {
@@ -301,27 +308,25 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                 if (!ok) break;
                 const uint32_t d = tmem + b * p.cols;
                 for (int kb = 0; kb < nkb; kb++) {
-                    if (BITS) ok = wait.spin(RFULL(r), rph);
-                    if (ok) ok = wait.spin(FULL(s), ph);
+                    if (BITS && !(ready & 2u)) ok = wait.spin(RFULL(r), rph);
+                    if (ok && !(ready & 1u)) ok = wait.spin(FULL(s), ph);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t lo = lo0 + (s * stage >> 4);
-                    mma_64<BITS, PAIRED>(leader, d, BITS ? tmem + ring_col + r * 32 : lo, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > 0);
-                    if (leader) {
-                        commit<PAIRED>(EMPTY(s));
-                        if (BITS) commit<PAIRED>(REMPTY(r));
-                        if (kb + 1 == nkb) commit<PAIRED>(SFULL(b));
-                    }
-                    __syncwarp();
+                    const uint32_t lo = lo0 + (s * stage >> 4), x = BITS ? tmem + ring_col + r * 32 : lo;
+                    const uint32_t bar_e = EMPTY(s), bar_r = REMPTY(r), bar_c = kb + 1 == nkb ? SFULL(b) : 0u;
                     if (++s == p.stages) { s = 0; ph ^= 1; }
                     if (BITS && ++r == p.ring) { r = 0; rph ^= 1; }
+                    ready = mma_64<BITS, PAIRED>(leader, d, x, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > 0, FULL(s), ph, RFULL(r), rph,
+                                                 bar_e, bar_r, bar_c);
                 }
                 if (++b == p.accumulators) { b = 0; bph ^= 1; }
             }
         if (!ok && leader) {
             // giving up: the MMAs already issued must have finished before tensor memory is freed
-            if constexpr (PAIRED) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(DRAIN) : "memory");
-            else mma_commit(DRAIN);
+            if constexpr (PAIRED)
+                asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(DRAIN) : "memory");
+            else
+                mma_commit(DRAIN);
             for (int i = 0; i < (1 << 20); i++)
                 if (PAIRED ? mbar_test_cluster(DRAIN, 0) : mbar_try_wait(DRAIN, 0)) break;
         }
