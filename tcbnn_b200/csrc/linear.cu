@@ -122,7 +122,7 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             p.accumulators = tiles <= teams || (bits && cols > 192) ? 1 : 2;
             p.ring = (512 - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
-            p.stages = (int)((226 * 1024 - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(p, bits));
+            p.stages = (int)((226 * 1024 - 8 * linear::kTurn - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(p, bits));
             if (p.stages > linear::kMaxStages) p.stages = linear::kMaxStages;
             while (linear::smem_bytes(p, bits) > 227 * 1024) p.stages--;
             const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;

@@ -4,7 +4,7 @@
 // The MMA's 128 rows are rows of W (outputs), its columns rows of x (tokens): one token costs 16 columns, a prompt 256,
 // by the same kernel, and what belongs to an output -- scale, bias, where it is stored -- belongs to a lane.
 //
-//   warps 0-7   epilogue  : lane = output, 32 tokens at a time
+//   warps 0-7   epilogue  : 32 outputs x 32 tokens at a time
 //   warp  8     loader W  : tensor copies of 128 rows x 64 (dense) or 128 rows x 512 bits (packed)
 //   warp  9     loader x  : tensor copies of `cols` rows x 64
 //   warp  10    MMA       : converged, elected lane; four MMAs of K = 16 per 64
@@ -28,6 +28,8 @@ constexpr int kThreadsDense = 11 * 32, kThreadsBits = 20 * 32;
 constexpr int kMaxCols = 256, kMaxStages = 12, kMaxRing = 8, kRawStages = 3;
 constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 rows of 64 elements, of 512 bits
 
+// 32 tokens x 32 outputs of 16 bits that an epilogue warp turns: rows of 64 bytes, 80 apart, so that eight of them meet different banks
+constexpr uint32_t kTurnPitch = 80, kTurn = 32 * kTurnPitch;
 enum Form { ALONE = 0, SPLIT = 1, PAIR = 2 };
 struct Plan {
     int form, cols, splits;                            // tokens per tile (a multiple of 16), CTAs that share K
@@ -44,7 +46,7 @@ __host__ __device__ inline size_t ring_bytes(const Plan& p, bool bits) {
     return ((ring > sums ? ring : sums) + 1023) & ~(size_t)1023;
 }
 __host__ __device__ inline size_t smem_bytes(const Plan& p, bool bits) {
-    return ring_bytes(p, bits) + (bits ? kRawStages * kRawStage : 0) + 64 * 8 + 1024;
+    return ring_bytes(p, bits) + (bits ? kRawStages * kRawStage : 0) + 8 * kTurn + 64 * 8 + 1024;
 }
 
 __device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -133,7 +135,29 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t shared, uint32_t rank) {
     return v;
 }
 
-// What a lane knows of its output, and how a sum becomes a result
+template <int COUNT>
+__device__ __forceinline__ void activate_all(float (&v)[COUNT], int activation) {
+    switch (activation) {
+    case RELU:
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], RELU);
+        break;
+    case GELU:
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU);
+        break;
+    case GELU_TANH:
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU_TANH);
+        break;
+    case SILU:
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], SILU);
+        break;
+    }
+}
+// Results of fp32, and the few of a cluster's CTA: a lane has its output's scale and bias, and stores token by token, a warp 128
+// (64) consecutive bytes.
 struct Output {
     const Args& a;
     int n;
@@ -147,24 +171,7 @@ struct Output {
     __device__ __forceinline__ void finish(float (&v)[COUNT], int m0, int rows) const {
 #pragma unroll
         for (int j = 0; j < COUNT; j++) v[j] = fmaf(v[j], scale, bias);
-        switch (a.activation) {
-        case RELU:
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], RELU);
-            break;
-        case GELU:
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU);
-            break;
-        case GELU_TANH:
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU_TANH);
-            break;
-        case SILU:
-#pragma unroll
-            for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], SILU);
-            break;
-        }
+        activate_all(v, a.activation);
         if (n >= a.N) return;
         if (a.residual) {
 #pragma unroll
@@ -174,6 +181,119 @@ struct Output {
 #pragma unroll
         for (int j = 0; j < COUNT; j++)
             if (j < rows) store(a.out, (m0 + j) * a.ldo + n, a.out_type, v[j]);
+    }
+};
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, int type) {
+    uint32_t w;
+    if (type == BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    return w;
+}
+__device__ __forceinline__ float2 unpack16(uint32_t w, int type) {
+    if (type == BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+// Results of 16 bits.  The sums come in pieces of 8 outputs x 8 tokens spread over a warp like an MMA's fragments, which stmatrix
+// stores turned, a token's eight outputs together; 16 bytes of a row are then a lane's, and a residual goes the other way.
+// (Two-byte stores, a lane an output: 16,000 clocks for 128 x 256.)
+struct Output16 {
+    const Args& a;
+    uint32_t turn;                                     // this warp's buffer
+    int n0;                                            // first of the warp's 32 outputs
+    bool wide_out, wide_res;                           // rows of 16-byte pieces
+    float scale[4], bias[4];                           // of outputs n0 + 8 i + lane / 4
+    __device__ __forceinline__ Output16(const Args& a_, uint32_t turn_, int n0_) : a(a_), turn(turn_), n0(n0_) {
+        wide_out = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.ldo * 2)) & 15) == 0;
+        wide_res = ((reinterpret_cast<uintptr_t>(a.residual) | (uintptr_t)(a.ldr * 2)) & 15) == 0;
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int n = n0 + 8 * i + (lane >> 2);
+            scale[i] = a.scale && n < a.N ? ld_dep(a.scale + n) : 1.f;
+            bias[i] = a.bias && n < a.N ? load(a.bias, n, a.bias_type) : 0.f;
+        }
+    }
+    // piece i of a lane: token m0 + 8 i + lane / 4, outputs n + 0..7
+    __device__ __forceinline__ void ask(uint4 (&r)[4], int m0, int rows) const {
+        const int lane = threadIdx.x & 31, n = n0 + 8 * (lane & 3);
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.residual) + n;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int j = 8 * i + (lane >> 2);
+            const uint16_t* q = p + (m0 + j) * a.ldr;
+            r[i] = make_uint4(0, 0, 0, 0);
+            if (j >= rows) continue;
+            if (wide_res && n + 8 <= a.N) {
+                r[i] = ld_dep(reinterpret_cast<const uint4*>(q));
+            } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = n + e < a.N ? q[e] : 0u;
+                r[i] = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+            }
+        }
+    }
+    // sums of 16 lanes (outputs) each as tmem_ld_16x256b_x4 gives them
+    __device__ __forceinline__ void finish(const int (&lo)[16], const int (&hi)[16], const uint4 (&r)[4], int m0, int rows) const {
+        const int lane = threadIdx.x & 31;
+        float v[32];
+#pragma unroll
+        for (int k = 0; k < 16; k++) {                   // register 4n + 2s + e: eight outputs s, token 8n + 2 (lane % 4) + e
+            const int s = (k >> 1) & 1;
+            v[k] = fmaf(__int_as_float(lo[k]), scale[s], bias[s]);
+            v[16 + k] = fmaf(__int_as_float(hi[k]), scale[2 + s], bias[2 + s]);
+        }
+        activate_all(v, a.activation);
+        const uint32_t piece = turn + (lane >> 2) * kTurnPitch + (lane & 3) * 16;       // a lane's 16 bytes
+        const uint32_t row = turn + (lane & 7) * kTurnPitch + (lane >> 3) * 16;          // a fragment's row
+        if (a.residual) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(piece + i * 8 * kTurnPitch), "r"(r[i].x), "r"(r[i].y), "r"(r[i].z), "r"(r[i].w) : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                uint32_t w[4];
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                             : "r"(row + n * 8 * kTurnPitch) : "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 f = unpack16(w[i], a.out_type);
+                    v[(i >> 1) * 16 + 4 * n + 2 * (i & 1)] += f.x;
+                    v[(i >> 1) * 16 + 4 * n + 2 * (i & 1) + 1] += f.y;
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(row + n * 8 * kTurnPitch),
+                         "r"(pack16(v[4 * n], v[4 * n + 1], a.out_type)), "r"(pack16(v[4 * n + 2], v[4 * n + 3], a.out_type)),
+                         "r"(pack16(v[16 + 4 * n], v[16 + 4 * n + 1], a.out_type)), "r"(pack16(v[16 + 4 * n + 2], v[16 + 4 * n + 3], a.out_type)) : "memory");
+        __syncwarp();
+        const int n = n0 + 8 * (lane & 3);
+        uint16_t* p = reinterpret_cast<uint16_t*>(a.out) + n;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int j = 8 * i + (lane >> 2);
+            if (j >= rows || n >= a.N) continue;
+            uint16_t* q = p + (m0 + j) * a.ldo;
+            const uint4 w = lds128(piece + i * 8 * kTurnPitch);
+            if (wide_out && n + 8 <= a.N) {
+                *reinterpret_cast<uint4*>(q) = w;
+            } else {
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (n + e < a.N) q[e] = (uint16_t)(x[e >> 1] >> (16 * (e & 1)));
+            }
+        }
+        __syncwarp();                                    // (the buffer is read)
     }
 };
 
@@ -188,7 +308,8 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     const uint32_t rank = CLUSTER || PAIRED ? [] { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }() : 0u;
     const uint32_t stage = stage_bytes(p, BITS);
     unsigned char* sRaw = smem + ring_bytes(p, BITS);
-    uint64_t* sBar = reinterpret_cast<uint64_t*>(sRaw + (BITS ? kRawStages * kRawStage : 0));
+    unsigned char* sTurn = sRaw + (BITS ? kRawStages * kRawStage : 0);
+    uint64_t* sBar = reinterpret_cast<uint64_t*>(sTurn + 8 * kTurn);
     // barriers: full[12] | empty[12] | ring full[8] | ring empty[8] | raw full[3] | raw empty[3] | sums full[2] | sums empty[2] | drain
     uint32_t* sTmem = reinterpret_cast<uint32_t*>(sBar + 51);
     volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
@@ -381,28 +502,48 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         for (int t = t_first; t < ntiles && ok; t += t_step) {
             int tm, tn;
             tile(t, tm, tn);
-            const Output out(a, tn * n_of + n_own + quad * 32 + lane);
-            if (nkb > 0) ok = wait.relaxed(SFULL(b), bph);
-            if (!ok) break;
-            tc_fence_after();
+            const int n0 = tn * n_of + n_own + quad * 32;
             const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + b * p.cols;
-            for (int c0 = half * 32; c0 < p.cols; c0 += 64) {
-                const int m0 = tm * p.cols + c0;
-                if (!CLUSTER && m0 >= a.M) break;
-                int v[32];
-                tmem_ld32(tcol + c0, v);
-                tmem_ld_wait();
-                float f[32];
+            if (!CLUSTER && a.out_type != FP32) {
+                const Output16 out(a, smem_u32(sTurn) + warp * kTurn, n0);
+                auto rows_of = [&](int c0) { return min(min(32, p.cols - c0), a.M - tm * p.cols - c0); };
+                uint4 res[4];
+                int c0 = half * 32;
+                if (a.residual && c0 < p.cols) out.ask(res, tm * p.cols + c0, rows_of(c0));
+                ok = wait.relaxed(SFULL(b), bph);
+                if (!ok) break;
+                tc_fence_after();
+                for (; c0 < p.cols && tm * p.cols + c0 < a.M; c0 += 64) {
+                    int lo[16], hi[16];
+                    tmem_ld_16x256b_x4(tcol + c0, lo);
+                    tmem_ld_16x256b_x4(tcol + (16u << 16) + c0, hi);
+                    tmem_ld_wait();
+                    out.finish(lo, hi, res, tm * p.cols + c0, rows_of(c0));
+                    if (a.residual && c0 + 64 < p.cols) out.ask(res, tm * p.cols + c0 + 64, rows_of(c0 + 64));
+                }
+            } else {
+                const Output out(a, n0 + lane);
+                if (nkb > 0) ok = wait.relaxed(SFULL(b), bph);
+                if (!ok) break;
+                tc_fence_after();
+                for (int c0 = half * 32; c0 < p.cols; c0 += 64) {
+                    const int m0 = tm * p.cols + c0;
+                    if (!CLUSTER && m0 >= a.M) break;
+                    int v[32];
+                    tmem_ld32(tcol + c0, v);
+                    tmem_ld_wait();
+                    float f[32];
 #pragma unroll
-                for (int j = 0; j < 32; j++) f[j] = nkb > 0 ? __int_as_float(v[j]) : 0.f;
-                if constexpr (CLUSTER) {
-                    // sums for the cluster: [four columns][128 outputs][4]
-                    float4* dst = reinterpret_cast<float4*>(smem) + (size_t)(c0 >> 2) * 128 + quad * 32 + lane;
+                    for (int j = 0; j < 32; j++) f[j] = nkb > 0 ? __int_as_float(v[j]) : 0.f;
+                    if constexpr (CLUSTER) {
+                        // sums for the cluster: [four columns][128 outputs][4]
+                        float4* dst = reinterpret_cast<float4*>(smem) + (size_t)(c0 >> 2) * 128 + quad * 32 + lane;
 #pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (c0 + 4 * j < p.cols) dst[j * 128] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-                } else {
-                    out.finish(f, m0, min(min(32, p.cols - c0), a.M - m0));
+                        for (int j = 0; j < 8; j++)
+                            if (c0 + 4 * j < p.cols) dst[j * 128] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                    } else {
+                        out.finish(f, m0, min(min(32, p.cols - c0), a.M - m0));
+                    }
                 }
             }
             tc_fence_before();                           // this warp is done with the sums
