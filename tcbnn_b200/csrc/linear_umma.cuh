@@ -8,7 +8,7 @@
 //   warp  8     loader W  : tensor copies of 128 rows x 64 (dense) or 128 rows x 512 bits (packed)
 //   warp  9     loader x  : tensor copies of `cols` rows x 64
 //   warp  10    MMA       : converged, elected lane; four MMAs of K = 16 per 64
-//   warps 12-19 expanders : (packed) two groups of four: signs to +-1 in tensor memory, where the MMA reads its W operand
+//   warps 12-15 expanders : (packed) signs to +-1 in tensor memory, where the MMA reads its W operand
 //
 // Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.  Packed weights cost a
 // sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port either.
@@ -24,7 +24,7 @@
 namespace tcbnn {
 namespace linear {
 
-constexpr int kThreadsDense = 11 * 32, kThreadsBits = 20 * 32;
+constexpr int kThreadsDense = 11 * 32, kThreadsBits = 16 * 32;
 constexpr int kMaxCols = 256, kMaxStages = 12, kMaxRing = 8, kRawStages = 3;
 constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 rows of 64 elements, of 512 bits
 
@@ -340,7 +340,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     if (tid == 0) {
         for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
         for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), PAIRED ? 8 : 4); mbar_init(REMPTY(s), 1); }
-        for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 8); }
+        for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 4); }
         for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), PAIRED ? 16 : 8); }
         mbar_init(DRAIN, 1);
         *sAbort = 0;
@@ -454,12 +454,20 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         __syncwarp();
     } else if (BITS && warp >= 12) {
         // =============================== expanders ==========================================
-        const int group = (warp - 12) >> 2, quad = warp & 3, row = quad * 32 + lane;
+        const int quad = warp & 3, row = quad * 32 + lane;
         const uint32_t minus = a.type == BF16 ? 0xBF80BF80u : 0xBC00BC00u;
         const uint32_t dst0 = tmem + ((uint32_t)(quad * 32) << 16) + ring_col;
-        int raw = 0, count = 0;                          // count: blocks of K in front, modulo two turns of the ring
-        uint32_t rawph = 0;
+        int raw = 0, r = 0, before = -1;                 // before: the slot being stored
+        uint32_t rawph = 0, rph = 0;
         bool ok = true;
+        auto hand_over = [&]() {
+            if (before < 0) return;
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(RFULL(before)); else mbar_arrive(RFULL(before)); }
+            before = -1;
+        };
         if (nkb > 0)
             for (int t = t_first; t < ntiles && ok; t += t_step)
                 for (int kb = 0; kb < nkb && ok; kb += 8) {
@@ -468,28 +476,23 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                     if (!ok) break;
                     // (the copy's 64-byte swizzle: 16-byte pieces turned by the row)
                     const uint32_t src = smem_u32(sRaw) + raw * kRawStage + row * 64;
-                    for (int j = group; j < blocks; j += 2) {
+                    for (int j = 0; j < blocks; j++) {
                         uint32_t w0, w1, e[32];
                         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w0), "=r"(w1)
                                      : "r"(src + (((j >> 1) ^ ((row >> 1) & 3)) << 4) + (j & 1) * 8) : "memory");
-                        expand_signs(w0, minus, e);
+                        expand_signs(w0, minus, e);      // (while the block in front is on its way)
                         expand_signs(w1, minus, e + 16);
-                        int at = count + j;
-                        if (at >= 2 * p.ring) at -= 2 * p.ring;
-                        const int r = at >= p.ring ? at - p.ring : at;
-                        ok = wait(REMPTY(r), at >= p.ring ? 0u : 1u);
+                        hand_over();
+                        ok = wait(REMPTY(r), rph ^ 1);
                         if (!ok) break;
                         tc_fence_after();
                         tmem_st32(dst0 + r * 32, e);
-                        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(RFULL(r)); else mbar_arrive(RFULL(r)); }
+                        before = r;
+                        if (++r == p.ring) { r = 0; rph ^= 1; }
                     }
+                    hand_over();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(RAWEMPTY(raw));
-                    count += blocks;
-                    if (count >= 2 * p.ring) count -= 2 * p.ring;
                     if (++raw == kRawStages) { raw = 0; rawph ^= 1; }
                 }
         __syncwarp();
@@ -499,6 +502,11 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         int b = 0;
         uint32_t bph = 0;
         bool ok = true;
+        auto give_back = [&](int of) {                   // this warp has what it needs of the sums
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(SEMPTY(of)); else mbar_arrive(SEMPTY(of)); }
+        };
         for (int t = t_first; t < ntiles && ok; t += t_step) {
             int tm, tn;
             tile(t, tm, tn);
@@ -506,20 +514,25 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + b * p.cols;
             if (!CLUSTER && a.out_type != FP32) {
                 const Output16 out(a, smem_u32(sTurn) + warp * kTurn, n0);
-                auto rows_of = [&](int c0) { return min(min(32, p.cols - c0), a.M - tm * p.cols - c0); };
+                const int m0 = tm * p.cols, cols = min(p.cols, a.M - m0);
+                const int n = (cols - half * 32 + 63) / 64;              // this warp's pieces of 32 tokens: every second one
+                auto at = [&](int k) { return half * 32 + k * 64; };
+                auto rows_of = [&](int k) { return min(32, cols - at(k)); };
                 uint4 res[4];
-                int c0 = half * 32;
-                if (a.residual && c0 < p.cols) out.ask(res, tm * p.cols + c0, rows_of(c0));
+                auto ask = [&](int k) { if (a.residual && k < n) out.ask(res, m0 + at(k), rows_of(k)); };
+                ask(0);
                 ok = wait.relaxed(SFULL(b), bph);
                 if (!ok) break;
                 tc_fence_after();
-                for (; c0 < p.cols && tm * p.cols + c0 < a.M; c0 += 64) {
+                if (n <= 0) give_back(b);
+                for (int k = 0; k < n; k++) {
                     int lo[16], hi[16];
-                    tmem_ld_16x256b_x4(tcol + c0, lo);
-                    tmem_ld_16x256b_x4(tcol + (16u << 16) + c0, hi);
+                    tmem_ld_16x256b_x4(tcol + at(k), lo);
+                    tmem_ld_16x256b_x4(tcol + (16u << 16) + at(k), hi);
                     tmem_ld_wait();
-                    out.finish(lo, hi, res, tm * p.cols + c0, rows_of(c0));
-                    if (a.residual && c0 + 64 < p.cols) out.ask(res, tm * p.cols + c0 + 64, rows_of(c0 + 64));
+                    if (k + 1 == n) give_back(b);        // (in front of the last piece's work)
+                    out.finish(lo, hi, res, m0 + at(k), rows_of(k));
+                    ask(k + 1);
                 }
             } else {
                 const Output out(a, n0 + lane);
@@ -546,9 +559,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                     }
                 }
             }
-            tc_fence_before();                           // this warp is done with the sums
-            __syncwarp();
-            if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(SEMPTY(b)); else mbar_arrive(SEMPTY(b)); }
+            if (CLUSTER || a.out_type == FP32) give_back(b);
             if (++b == p.accumulators) { b = 0; bph ^= 1; }
         }
     }
