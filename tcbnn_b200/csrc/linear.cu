@@ -13,7 +13,7 @@ namespace {
 __device__ int g_linear_status;      // 1 after a bounded wait inside k_linear gave up
 
 template <bool BITS, int FORM>
-__global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, 1)
+__global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, FORM == linear::SPLIT ? 2 : 1)
 k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
     linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
@@ -120,11 +120,18 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
             p.accumulators = tiles <= teams || (bits && cols > 192) ? 1 : 2;
-            p.ring = (512 - p.accumulators * cols) / 32;
+            // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
+            const bool half = p.form == linear::SPLIT;
+            p.ring = (half ? 256 - cols > 128 ? 256 - cols : 128 : 512 - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
-            p.stages = (int)((226 * 1024 - 8 * linear::kTurn - (bits ? linear::kRawStages * linear::kRawStage : 0)) / linear::stage_bytes(p, bits));
+            p.columns = 32;
+            while (p.columns < p.accumulators * cols + (bits ? 32 * p.ring : 0)) p.columns *= 2;
+            const int room = (half ? 113 : 227) * 1024;
+            p.stages = (room - 2048 - 8 * (int)linear::kTurn - (bits ? linear::kRawStages * (int)linear::kRawStage : 0)) / (int)linear::stage_bytes(p, bits);
             if (p.stages > linear::kMaxStages) p.stages = linear::kMaxStages;
-            while (linear::smem_bytes(p, bits) > 227 * 1024) p.stages--;
+            if (p.stages < 2) p.stages = 2;
+            while (p.stages > 2 && linear::smem_bytes(p, bits) > (size_t)room) p.stages--;
+            if (linear::smem_bytes(p, bits) > 227 * 1024) continue;
             const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;
             double block = bytes / 72 > mma ? bytes / 72 : mma;
             if (bits && block < 130) block = 130;

@@ -36,6 +36,7 @@ struct Plan {
     int tiles_m, tiles_n, band;                        // tiles of tokens and of outputs; token tiles worked on together
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
+    int columns;                                       // of tensor memory
 };
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
@@ -337,6 +338,10 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         tm = b * p.band + r - tn * w;
     };
 
+    if (warp == 8 && lane == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map_x) : "memory");
+    }
     if (tid == 0) {
         for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
         for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), PAIRED ? 8 : 4); mbar_init(REMPTY(s), 1); }
@@ -348,10 +353,10 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     }
     if (warp == 10) {
         if constexpr (PAIRED) {
-            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(sTmem)), "r"(p.columns) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         } else {
-            tmem_alloc(smem_u32(sTmem), 512);
+            tmem_alloc(smem_u32(sTmem), p.columns);
         }
     }
     fence_proxy_async();
@@ -592,9 +597,9 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     __syncthreads();
     if constexpr (PAIRED) {
         cluster_sync();                                  // nothing of the partner's reaches into this CTA any more
-        if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns) : "memory");
     } else if (warp == 10) {
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, p.columns);
     }
 }
 
