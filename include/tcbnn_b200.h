@@ -416,7 +416,7 @@ int tcbnn_linear(const void* x, const void* W, const void* bias, const void* res
                  size_t workspace_bytes, void* stream);
 /* The same with binary weights: out = act(scale[n] * sum_k x[m][k] * w[n][k] + bias[n]) + residual[m][n], w[n][k] = +-1 the packed
  * bits of row n (tcbnn_pack_fc_weight; ldw in words, a multiple of 4, 16-byte aligned; bits behind element K may be anything),
- * scale [N] fp32 or NULL for 1.  Workspace as above with W = NULL. */
+ * scale [N] fp32 or NULL for 1.  Workspace as above with W = NULL; few rows need none. */
 int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const void* bias, const void* residual, void* out, int M,
                      int N, int K, long long ldx, long long ldw, long long ldr, long long ldo, int type, int out_type, int bias_type,
                      int activation, void* workspace, size_t workspace_bytes, void* stream);
@@ -424,7 +424,9 @@ int tcbnn_bit_linear(const void* x, const uint32_t* W, const float* scale, const
  * gave up and results since the last reading are not valid; reading a failure clears it). */
 int tcbnn_linear_status(int* status);
 /* Forces their tiles of `cols` tokens (16 to 256 in steps of 16) and the CTAs (1, 2, 4 or 8) that share K, or with splits = -2
- * pairs of CTAs that share tiles of 256 outputs (cols in steps of 32); 0 = automatic.  Process-wide; for tests and measurements. */
+ * pairs of CTAs that share tiles of 256 outputs (cols in steps of 32); 0 = automatic.  Packed weights have no pairs, and share K in tiles
+ * of up to 128 tokens; a forced plan also keeps few rows off the kernel on warp-level MMAs.  Calls without the forced plan fail.
+ * Process-wide; for tests and measurements. */
 int tcbnn_set_linear_plan(int cols, int splits);
 /* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);

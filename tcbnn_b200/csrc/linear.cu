@@ -3,7 +3,7 @@
 #include <cmath>
 #include "host.cuh"
 #include "bnn_layers.cuh"
-#include "linear_umma.cuh"
+#include "bit_linear_small.cuh"
 #include "log_probs.cuh"
 
 using namespace tcbnn;
@@ -18,10 +18,17 @@ k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CU
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
     linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
 }
-__global__ void __launch_bounds__(256) k_repack(const uint16_t* src, long long ld, int rows, int K, int pitch, uint16_t* dst) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the product waits before it reads)
-    linear::repack(src, ld, rows, K, pitch, dst);
+template <int RT, bool BF>
+__global__ void __launch_bounds__(32 * linear::kSmallWarps, 1) k_bit_linear_small(linear::Args a) {
+    extern __shared__ __align__(16) float bit_linear_sums[];
+    linear::bit_linear_small<RT, BF>(a, bit_linear_sums);
 }
+__global__ void __launch_bounds__(256) k_repack(linear::Rows x, linear::Rows w, int K) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    linear::repack(x, w, K);
+}
+
 template <int TYPE, int NW, bool CLUSTER>
 __global__ void __launch_bounds__(NW == 1 ? 256 : NW * 32, 32 / (NW == 1 ? 8 : NW)) k_log_probs(scores::Args a) {
     __shared__ scores::Shared<NW> shared[NW == 1 ? 8 : 1];
@@ -93,22 +100,46 @@ size_t packed_bytes(int rows, int K) { return ((size_t)rows * ((K + 7) & ~7) * 2
 
 int g_linear_cols = 0, g_linear_splits = 0;              // tcbnn_set_linear_plan: 0 = from the model
 
-// The plan with the least clocks.  A block of 64 of K costs a CTA its MMAs (cols / 2 each), its bytes from L2, or, with packed
-// weights, the expanders' time; a tile its set-up and what of the epilogue shows; a cluster its exchange.
+// What a plan takes, in us at 1.9 GHz, fitted to 1400 forced plans over 22 shapes: the set-up of a launch, of a cluster's exchange, of a
+// pair; a wave of tiles, each its blocks of 64 of K -- MMAs of cols / 2 clocks, or the bytes that a CTA draws from L2, or its
+// expanders -- and an epilogue that the next tile's blocks hide but for a share; no less than the operands' way from memory.
+double plan_time(const linear::Plan& p, int M, int N, int K, int sms) {
+    struct Fit { double start, split[4], pair, clocks, bytes, block, finish, column, shown, memory; };
+    static const Fit of[2] = {{2.2, {0, 3.0, 2.0, 1.7}, 1.4, 1.03, 72, 0, 2590, 30, 0.36, 5800},
+                              {3.6, {0, 2.2, 1.9, 1.5}, 0, 1.03, 59, 500, 1760, 24, 0.44, 4700}};
+    const Fit& f = of[p.bits];
+    const bool pair = p.form == linear::PAIR;
+    const double tiles = (double)p.tiles_m * p.tiles_n, bytes = (p.bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;
+    double waves = ceil(tiles * p.splits / (pair ? sms / 2 : sms)), block = 2.0 * p.cols * f.clocks;
+    if (block < bytes / f.bytes) block = bytes / f.bytes;
+    if (p.splits > 1 && waves > 1) {                     // (two CTAs share an SM, but not each other's latency)
+        block *= 2;
+        waves = ceil(waves / 2);
+    }
+    if (block < f.block) block = f.block;
+    const double finish = f.finish + f.column * p.cols, blocks = p.per < p.kblocks ? p.per : p.kblocks;
+    const double clocks = waves * (blocks * block + finish * (p.accumulators == 1 ? 1 : f.shown)) + (p.accumulators == 1 ? 0 : finish);
+    const double weight = p.bits ? N * (K / 8.0) : 2.0 * N * K;
+    const double memory = (weight + 2.0 * M * K + 2.0 * M * N) / (f.memory * 1e3);
+    return (clocks / 1900 > memory ? clocks / 1900 : memory) + f.start + (pair ? f.pair : f.split[p.splits == 8 ? 3 : p.splits / 2]);
+}
+
+// The plan that takes least.
 linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
     linear::Plan best = {};
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
-    for (int shape = 0; shape < 5; shape++) {
+    for (int shape = 0; shape < (bits ? 4 : 5); shape++) {               // K in 1, 2, 4, 8; pairs of CTAs
         const bool pair = shape == 4;
         const int splits = pair ? 1 : 1 << shape;
         if (g_linear_splits && g_linear_splits != (pair ? -2 : splits)) continue;
         const int per = ((kblocks + splits - 1) / splits + unit - 1) / unit * unit;
         if (splits > 1 && (splits - 1) * per >= kblocks && !g_linear_splits) continue;       // (a CTA without work)
-        const int teams = pair || splits == 2 ? sms / 2 : splits == 1 ? sms : splits == 4 ? sms * 33 / 148 : sms * 15 / 148;
         for (int cols = pair ? 32 : 16; cols <= linear::kMaxCols; cols += pair ? 32 : 16) {
             linear::Plan p = {};
+            p.bits = bits;
             p.form = pair ? linear::PAIR : splits > 1 ? linear::SPLIT : linear::ALONE;
+            if (bits && splits > 1 && cols > 128) continue;
             p.cols = cols;
             p.splits = splits;
             p.tiles_m = (M + cols - 1) / cols;
@@ -119,25 +150,17 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             p.kblocks = kblocks;
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
-            p.accumulators = tiles <= teams || (bits && cols > 192) ? 1 : 2;
-            // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
-            const bool half = p.form == linear::SPLIT;
-            p.ring = (half ? 256 - cols > 128 ? 256 - cols : 128 : 512 - p.accumulators * cols) / 32;
+            // a second set of sums where there is room, and a second tile
+            p.accumulators = tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192) ? 1 : 2;
+            p.ring = !bits ? 0 : ((p.form == linear::SPLIT ? 256 : 512) - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
             p.columns = 32;
-            while (p.columns < p.accumulators * cols + (bits ? 32 * p.ring : 0)) p.columns *= 2;
-            const int room = (half ? 113 : 227) * 1024;
-            p.stages = (room - 2048 - 8 * (int)linear::kTurn - (bits ? linear::kRawStages * (int)linear::kRawStage : 0)) / (int)linear::stage_bytes(p, bits);
-            if (p.stages > linear::kMaxStages) p.stages = linear::kMaxStages;
-            if (p.stages < 2) p.stages = 2;
-            while (p.stages > 2 && linear::smem_bytes(p, bits) > (size_t)room) p.stages--;
-            if (linear::smem_bytes(p, bits) > 227 * 1024) continue;
-            const double mma = 2.0 * cols, bytes = (bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;
-            double block = bytes / 72 > mma ? bytes / 72 : mma;
-            if (bits && block < 130) block = 130;
-            const double finish = 400 + cols * 12.0, waves = (double)((tiles + teams - 1) / teams);
-            const double clocks = waves * (p.per * block + (p.accumulators == 1 ? finish : 200)) + finish + 2500 + (splits > 1 || pair ? 2000 : 0);
-            if (clocks < least) { least = clocks; best = p; }
+            while (p.columns < p.accumulators * cols + 32 * p.ring) p.columns *= 2;
+            // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
+            const size_t room = (p.form == linear::SPLIT ? 113 : 227) * 1024;
+            for (p.stages = linear::kMaxStages; p.stages > 2 && linear::smem_bytes(p) > room; p.stages--) {}
+            const double t = plan_time(p, M, N, K, sms);
+            if (t < least) { least = t; best = p; }
         }
     }
     return best;
@@ -153,6 +176,14 @@ const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
     return k.plan;
 }
 
+// Packed weights and few rows: whether the kernel on warp-level MMAs is the faster one.  It takes 2.8 us and what its expansions take,
+// 6.5e6 weights a us for every eight rows (8192 x 8192 for 24 rows 34 us, 4096 x 4096 for 32 13, for one 4.1; the other kernel 17.5, 9.5, 8.6).
+bool small_pays(int M, int N, int K, int sms) {
+    if (M > 128 || g_linear_cols || g_linear_splits) return false;
+    const double us = 2.8 + (double)((M + 7) / 8) * N * K / 6.5e6;
+    return us < plan_time(plan_linear(M, N, K, true, sms), M, N, K, sms);
+}
+
 int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int width, int rows, long long pitch_bytes, int box_x, int box_y,
                CUtensorMapSwizzle swizzle) {
     if (!tensor_encode()) return fail("linear: the driver has no cuTensorMapEncodeTiled");
@@ -165,27 +196,68 @@ int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int
     return 0;
 }
 
-template <bool BITS>
 int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const CUtensorMap& map_w, const CUtensorMap& map_x, cudaStream_t st) {
+    using namespace linear;
+    using Kernel = void (*)(Args, Plan, int*, CUtensorMap, CUtensorMap);
+    static const struct { bool bits; int form; Kernel kernel; } of[] = {
+        {false, ALONE, k_linear<false, ALONE>}, {false, SPLIT, k_linear<false, SPLIT>}, {false, PAIR, k_linear<false, PAIR>},
+        {true, ALONE, k_linear<true, ALONE>}, {true, SPLIT, k_linear<true, SPLIT>}};
     static bool done[64];
-    if (configure_once(done, [] {
-            cudaError_t e = cudaFuncSetAttribute(k_linear<BITS, linear::ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(k_linear<BITS, linear::SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-            return e != cudaSuccess ? e : cudaFuncSetAttribute(k_linear<BITS, linear::PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    static int* status_of[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configure_once(done, [&] {
+            cudaError_t e = cudaSuccess;
+            for (const auto& k : of)
+                if (e == cudaSuccess) e = cudaFuncSetAttribute(k.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            return e != cudaSuccess ? e : cudaGetSymbolAddress((void**)&status_of[dev & 63], g_linear_status);
         })) return 1;
-    void* status = nullptr;
-    CUDA_TRY(cudaGetSymbolAddress(&status, g_linear_status));
+    int i = 0;
+    while (of[i].bits != (bool)p.bits || of[i].form != p.form) i++;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
-    const int threads = BITS ? linear::kThreadsBits : linear::kThreadsDense;
-    const size_t smem = linear::smem_bytes(p, BITS);
-    const int team = p.form == linear::PAIR ? 2 : p.splits;
-    const long long teams = p.form == linear::SPLIT || tiles < sms / team ? tiles : sms / team;
-    auto kernel = p.form == linear::ALONE ? k_linear<BITS, linear::ALONE> : p.form == linear::SPLIT ? k_linear<BITS, linear::SPLIT>
-                                                                                                    : k_linear<BITS, linear::PAIR>;
-    const cudaError_t e = launch_dependent_cluster(kernel, (unsigned)(teams * team), team > 1 ? team : 0, threads, smem, st, a, p, (int*)status,
-                                                   map_w, map_x);
+    const int team = p.form == PAIR ? 2 : p.splits;
+    const long long teams = p.form == SPLIT || tiles < sms / team ? tiles : sms / team;
+    const cudaError_t e = launch_dependent_cluster(of[i].kernel, (unsigned)(teams * team), team > 1 ? team : 0, p.bits ? kThreadsBits : kThreadsDense, smem_bytes(p), st,
+                                                   a, p, status_of[dev & 63], map_w, map_x);
     if (e != cudaSuccess) return fail("linear: %s", cudaGetErrorString(e));
     return 0;
+}
+
+int run_bit_linear_small(const linear::Args& a, int sms, cudaStream_t st) {
+    using namespace linear;
+    using Kernel = void (*)(Args);
+    static const struct { int rt; Kernel bf16, fp16; } of[] = {
+#define TCBNN_SMALL(RT) {RT, k_bit_linear_small<RT, true>, k_bit_linear_small<RT, false>}
+        TCBNN_SMALL(1), TCBNN_SMALL(2), TCBNN_SMALL(4)};
+#undef TCBNN_SMALL
+    static bool done[64];
+    if (configure_once(done, [] {
+            cudaError_t e = cudaSuccess;
+            for (const auto& k : of)
+                for (Kernel f : {k.bf16, k.fp16})
+                    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small_bytes(k.rt, kSmallWarps));
+            return e;
+        })) return 1;
+    const int pieces = (a.K + 255) / 256;
+    // 16 x RT outputs per block: as many as still give every SM a block.  Sixteen warps where a block has its SM to itself: 1 x 4096 x
+    // 4096 4.1 us with RT = 2, 5.7 with 1, 6.1 with eight warps; 1 x 16384 x 4096 11.6 with RT = 4 and eight, 13.0 with sixteen.
+    const int i = a.N <= 16 * sms ? 0 : a.N <= 32 * sms ? 1 : 2, rt = of[i].rt;
+    const long long blocks = (long long)((a.N + 16 * rt - 1) / (16 * rt)) * ((a.M + 7) / 8);
+    int warps = blocks <= sms ? kSmallWarps : kSmallWarps / 2;
+    if (warps > pieces) warps = pieces;
+    const dim3 grid((a.N + 16 * rt - 1) / (16 * rt), (a.M + 7) / 8);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(32 * warps);
+    cfg.dynamicSmemBytes = small_bytes(rt, warps);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, a.type == TCBNN_BF16 ? of[i].bf16 : of[i].fp16, a);
+    return e != cudaSuccess ? fail("bit_linear: %s", cudaGetErrorString(e)) : 0;
 }
 
 int run_linear(const char* what, linear::Args a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {
@@ -193,30 +265,35 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     if (a.M == 0) return 0;
     int sms;
     if (sm_count(&sms)) return 1;
+    if (bits && small_pays(a.M, a.N, a.K, sms)) return run_bit_linear_small(a, sms, st);
     const size_t need = tcbnn_linear_workspace_bytes(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
     if (need) {
         if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
             return fail("%s: these operands need %zu bytes of workspace, 256-byte aligned", what, need);
         char* room = (char*)workspace;
-        const int pitch = (a.K + 7) & ~7;
-        auto repack = [&](const void** p, long long* ld, int rows) {
-            const long long units = (long long)rows * (pitch / 8), blocks = (units + 255) / 256;
-            k_repack<<<(unsigned)(blocks < 16LL * sms ? blocks : 16LL * sms), 256, 0, st>>>((const uint16_t*)*p, *ld, rows, a.K, pitch, (uint16_t*)room);
+        linear::Rows moved[2] = {};
+        long long units = 0;
+        const auto move = [&](linear::Rows& m, const void** p, long long* ld, int rows) {
+            m = linear::Rows{(const uint16_t*)*p, (uint16_t*)room, *ld, rows};
             *p = room;
-            *ld = pitch;
+            *ld = (a.K + 7) & ~7;
             room += packed_bytes(rows, a.K);
+            units += (long long)rows * ((a.K + 7) / 8);
         };
-        if (!rows_fit(a.x, a.ldx, a.M)) repack(&a.x, &a.ldx, a.M);
-        if (!bits && !rows_fit(a.W, a.ldw, a.N)) repack(&a.W, &a.ldw, a.N);
-        if (launch_check(what)) return 1;
+        if (!rows_fit(a.x, a.ldx, a.M)) move(moved[0], &a.x, &a.ldx, a.M);
+        if (!bits && !rows_fit(a.W, a.ldw, a.N)) move(moved[1], &a.W, &a.ldw, a.N);
+        const long long blocks = (units + 255) / 256;
+        const cudaError_t e = launch_dependent(k_repack, (unsigned)(blocks < 16LL * sms ? blocks : 16LL * sms), 256, 0, st, moved[0], moved[1], a.K);
+        if (e != cudaSuccess) return fail("%s: %s", what, cudaGetErrorString(e));
     }
     const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, sms);
+    if (!p.cols) return fail("%s: the forced plan does not exist for these operands", what);
     const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap map_w, map_x;
     if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, linear::own_cols(p), CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
     if (bits ? linear_map(&map_w, a.W, CU_TENSOR_MAP_DATA_TYPE_UINT32, (a.K + 31) / 32, a.N, a.ldw * 4, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B)
              : linear_map(&map_w, a.W, type, a.K, a.N, a.ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
-    return bits ? launch_linear<true>(a, p, sms, map_w, map_x, st) : launch_linear<false>(a, p, sms, map_w, map_x, st);
+    return launch_linear(a, p, sms, map_w, map_x, st);
 }
 
 int g_scores_warps = 0, g_scores_ctas = 0;               // tcbnn_set_log_probs_plan: 0 = from the sizes
@@ -255,7 +332,8 @@ int run_log_probs(const scores::Args& a, int sms, cudaStream_t st) {
 extern "C" {
 
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw) {
-    if (M < 1 || N < 1 || K < 1) return 0;
+    int sms;
+    if (M < 1 || N < 1 || K < 1 || (!W && !sm_count(&sms) && small_pays(M, N, K, sms))) return 0;
     return (rows_fit(x, ldx, M) ? 0 : packed_bytes(M, K)) + (!W || rows_fit(W, ldw, N) ? 0 : packed_bytes(N, K));
 }
 

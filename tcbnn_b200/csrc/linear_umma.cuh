@@ -32,7 +32,7 @@ constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 
 constexpr uint32_t kTurnPitch = 80, kTurn = 32 * kTurnPitch;
 enum Form { ALONE = 0, SPLIT = 1, PAIR = 2 };
 struct Plan {
-    int form, cols, splits;                            // tokens per tile (a multiple of 16), CTAs that share K
+    int bits, form, cols, splits;                            // tokens per tile (a multiple of 16), CTAs that share K
     int tiles_m, tiles_n, band;                        // tiles of tokens and of outputs; token tiles worked on together
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
@@ -40,14 +40,14 @@ struct Plan {
 };
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
-__host__ __device__ inline uint32_t stage_bytes(const Plan& p, bool bits) { return (bits ? 0u : kWStage) + (uint32_t)own_cols(p) * 128u; }
+__host__ __device__ inline uint32_t stage_bytes(const Plan& p) { return (p.bits ? 0u : kWStage) + (uint32_t)own_cols(p) * 128u; }
 // ring (where the cluster's sums go afterwards), raw bits, barriers; 1 KB for its alignment
-__host__ __device__ inline size_t ring_bytes(const Plan& p, bool bits) {
-    const size_t ring = (size_t)p.stages * stage_bytes(p, bits), sums = p.splits > 1 ? (size_t)p.cols * 512 : 0;
+__host__ __device__ inline size_t ring_bytes(const Plan& p) {
+    const size_t ring = (size_t)p.stages * stage_bytes(p), sums = p.splits > 1 ? (size_t)p.cols * 512 : 0;
     return ((ring > sums ? ring : sums) + 1023) & ~(size_t)1023;
 }
-__host__ __device__ inline size_t smem_bytes(const Plan& p, bool bits) {
-    return ring_bytes(p, bits) + (bits ? kRawStages * kRawStage : 0) + 8 * kTurn + 64 * 8 + 1024;
+__host__ __device__ inline size_t smem_bytes(const Plan& p) {
+    return ring_bytes(p) + (p.bits ? kRawStages * kRawStage : 0) + (p.form != SPLIT ? 8 * kTurn : 0) + 64 * 8 + 1024;
 }
 
 __device__ __forceinline__ void tensor_g2s(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
@@ -304,13 +304,14 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     using namespace umma;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem0) + 1023) & ~(uintptr_t)1023);
     constexpr bool CLUSTER = FORM == SPLIT, PAIRED = FORM == PAIR;
+    static_assert(!BITS || !PAIRED, "no pairs with packed weights: they were no faster");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t nctas = CLUSTER ? [] { uint32_t n; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }() : 1u;
     const uint32_t rank = CLUSTER || PAIRED ? [] { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }() : 0u;
-    const uint32_t stage = stage_bytes(p, BITS);
-    unsigned char* sRaw = smem + ring_bytes(p, BITS);
+    const uint32_t stage = stage_bytes(p);
+    unsigned char* sRaw = smem + ring_bytes(p);
     unsigned char* sTurn = sRaw + (BITS ? kRawStages * kRawStage : 0);
-    uint64_t* sBar = reinterpret_cast<uint64_t*>(sTurn + 8 * kTurn);
+    uint64_t* sBar = reinterpret_cast<uint64_t*>(sTurn + (CLUSTER ? 0 : 8 * kTurn));
     // barriers: full[12] | empty[12] | ring full[8] | ring empty[8] | raw full[3] | raw empty[3] | sums full[2] | sums empty[2] | drain
     uint32_t* sTmem = reinterpret_cast<uint32_t*>(sBar + 51);
     volatile int* sAbort = reinterpret_cast<volatile int*>(sTmem + 1);
@@ -344,7 +345,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     }
     if (tid == 0) {
         for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
-        for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), PAIRED ? 8 : 4); mbar_init(REMPTY(s), 1); }
+        for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), 4); mbar_init(REMPTY(s), 1); }
         for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 4); }
         for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), PAIRED ? 16 : 8); }
         mbar_init(DRAIN, 1);
@@ -470,7 +471,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(RFULL(before)); else mbar_arrive(RFULL(before)); }
+            if (lane == 0) mbar_arrive(RFULL(before));
             before = -1;
         };
         if (nkb > 0)
@@ -603,18 +604,21 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     }
 }
 
-// Rows of K elements of 16 bits, any distance apart, to rows of `pitch` elements
-__device__ __forceinline__ void repack(const uint16_t* src, long long ld, int rows, int K, int pitch, uint16_t* dst) {
-    const long long total = (long long)rows * (pitch / 8);
+// Rows of K elements of 16 bits, any distance apart, copied to rows of a multiple of 8 elements (none where rows = 0)
+struct Rows { const uint16_t* from; uint16_t* to; long long ld; int rows; };
+__device__ __forceinline__ void repack(const Rows& x, const Rows& w, int K) {
+    const int pieces = (K + 7) / 8;
+    const long long of_x = (long long)x.rows * pieces, total = of_x + (long long)w.rows * pieces;
     for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-        const long long r = i / (pitch / 8);
-        const int k = (int)(i - r * (pitch / 8)) * 8;
-        const uint16_t* s = src + r * ld + k;
-        uint32_t w[4];
+        const bool isw = i >= of_x;
+        const long long j = isw ? i - of_x : i, r = j / pieces;
+        const int k = (int)(j - r * pieces) * 8;
+        const uint16_t* s = isw ? w.from + r * w.ld + k : x.from + r * x.ld + k;
+        uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            w[j] = (k + 2 * j < K ? (uint32_t)s[2 * j] : 0u) | (k + 2 * j + 1 < K ? (uint32_t)s[2 * j + 1] << 16 : 0u);
-        reinterpret_cast<uint4*>(dst + r * pitch + k)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int q = 0; q < 4; q++)
+            v[q] = (k + 2 * q < K ? (uint32_t)s[2 * q] : 0u) | (k + 2 * q + 1 < K ? (uint32_t)s[2 * q + 1] << 16 : 0u);
+        reinterpret_cast<uint4*>(isw ? w.to : x.to)[j] = make_uint4(v[0], v[1], v[2], v[3]);
     }
 }
 

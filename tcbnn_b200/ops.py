@@ -253,10 +253,9 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
 
 
 def linear_workspace(x, weight):
-    """Scratch that linear() needs on these operands (bit_linear(): weight=None), or None; without one given it is
-    allocated per call."""
-    N, ldw = (1, 8) if weight is None else (weight.shape[0], weight.stride(0))
-    n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), _ptr(weight), x.shape[0], N, x.shape[1], x.stride(0), ldw)
+    """Scratch that linear() or bit_linear() needs on these operands, or None; without one given it is allocated per call."""
+    bits = weight.dtype is torch.int32
+    n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), None if bits else _ptr(weight), x.shape[0], weight.shape[0], x.shape[1], x.stride(0), weight.stride(0))
     return torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
 
 

@@ -94,6 +94,13 @@ def test_every_plan(cuda, bits, cols, splits, M, N, K):
     x, w, scale, sums = case(bits, M, N, K, BF16, cuda)
     bias, res = whole(gen(M), (N,), 50, FP32, cuda), whole(gen(N), (M, N), 50, FP32, cuda)
     ops.set_linear_plan(cols, splits)
+    if bits and (splits == -2 or (splits > 1 and cols > 128)):           # (no such kernel)
+        try:
+            with pytest.raises(lib.TcbnnError):
+                product(bits, x, w, scale)
+        finally:
+            ops.set_linear_plan()
+        return
     try:
         got = product(bits, x, w, scale, bias, "relu", res, out_dtype=FP32)
         assert ops.linear_status() == 0
@@ -173,6 +180,21 @@ def test_rows_apart_and_what_lies_between_them(cuda, bits, dtype, M, N, K, pad):
         product(bits, x, w, scale, residual=r, out=r)
         assert torch.equal(r.double(), sums + 5)
         assert (rbuf[mask] == 5.0).all()
+
+
+@pytest.mark.parametrize("bits", [False, True])
+@pytest.mark.parametrize("M,N,K", [(3, 50, 77), (500, 600, 333)])
+def test_workspaces(cuda, bits, M, N, K):
+    """A workspace of one's own, for operands that need one; too small ones and none are refused by the library."""
+    x, w, scale, sums = case(bits, M, N, K, BF16, cuda)
+    ws = ops.linear_workspace(x, w)
+    assert (ws is None) == (bits and M == 3)           # (few rows of packed weights are read where they lie)
+    assert torch.equal(product(bits, x, w, scale, out_dtype=FP32, workspace=ws).double(), sums)
+    aligned = torch.zeros((M, 80 if K == 77 else 336), dtype=BF16, device=cuda)
+    assert ops.linear_workspace(aligned, w if bits else aligned) is None
+    if ws is not None:
+        with pytest.raises(lib.TcbnnError):
+            product(bits, x, w, scale, workspace=ws[:-256])
 
 
 @pytest.mark.parametrize("bits", [False, True])
