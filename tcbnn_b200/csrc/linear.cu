@@ -145,7 +145,7 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             p.tiles_m = (M + cols - 1) / cols;
             p.tiles_n = pair ? (N + 255) / 256 : (N + 127) / 128;
             const long long tiles = (long long)p.tiles_m * p.tiles_n;
-            if (splits > 1 && tiles * splits > (1 << 20)) continue;
+            if (splits > 1 && tiles * splits > (g_linear_splits ? 1 << 20 : 3LL * sms)) continue;      // (as far as the times were fitted)
             if (g_linear_cols ? cols != g_linear_cols : cols > 32 && cols >= M + 32) continue;
             p.kblocks = kblocks;
             p.per = per;
