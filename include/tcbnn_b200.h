@@ -408,7 +408,7 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
  * (or NULL) and out [M][ldo] of `type` or fp32 (out_type).  Leading dimensions count elements; what lies between rows is neither
  * read nor written.  Sums, activation and residual are fp32, the result is rounded once.
  * residual may be out itself (same pointer and leading dimension); otherwise out shares no memory with an input.
- * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for large operands whose rows do not all start on 16 bytes (they
+ * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for operands whose rows do not all start on 16 bytes (they
  * are copied to rows that do; 0 for others).  Calls that may run at the same time need workspaces of their own. */
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw);
 int tcbnn_linear(const void* x, const void* W, const void* bias, const void* residual, void* out, int M, int N, int K, long long ldx,
@@ -428,9 +428,6 @@ int tcbnn_linear_status(int* status);
  * of up to 128 tokens; a forced plan also keeps few rows off the kernel on warp-level MMAs.  Calls without the forced plan fail.
  * Process-wide; for tests and measurements. */
 int tcbnn_set_linear_plan(int cols, int splits);
-/* Operands whose rows do not all start on 16 bytes: 1 = copied first (workspace), 2 = turned by the product's own loaders, 0 =
- * automatic.  Process-wide; for tests and measurements. */
-int tcbnn_set_linear_copy(int copy);
 /* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
  *                                            0 for a negative target (a row without one), NaN for one past V - 1

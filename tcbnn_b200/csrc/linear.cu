@@ -12,12 +12,11 @@ namespace {
 
 __device__ int g_linear_status;      // 1 after a bounded wait inside k_linear gave up
 
-// (a CTA of a cluster leaves room for another, see make_plan, but for the loaders of loose operands)
-template <bool BITS, int FORM, bool LOOSE>
-__global__ void __launch_bounds__(linear::threads_of(BITS, LOOSE), FORM == linear::SPLIT && !LOOSE ? 2 : 1)
+template <bool BITS, int FORM>
+__global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, FORM == linear::SPLIT ? 2 : 1)
 k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
-    linear::umma_cta<BITS, FORM, LOOSE>(a, p, &map_w, &map_x, status, dyn_smem_linear);
+    linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
 }
 template <int RT, bool BF>
 __global__ void __launch_bounds__(32 * linear::kSmallWarps, 1) k_bit_linear_small(linear::Args a) {
@@ -113,14 +112,11 @@ double plan_time(const linear::Plan& p, int M, int N, int K, int sms) {
     const double tiles = (double)p.tiles_m * p.tiles_n, bytes = (p.bits ? 1024 : 16384) + linear::own_cols(p) * 128.0;
     double waves = ceil(tiles * p.splits / (pair ? sms / 2 : sms)), block = 2.0 * p.cols * f.clocks;
     if (block < bytes / f.bytes) block = bytes / f.bytes;
-    if (p.splits > 1 && waves > 1 && !p.loose) {                     // (two CTAs share an SM, but not each other's latency)
+    if (p.splits > 1 && waves > 1) {                     // (two CTAs share an SM, but not each other's latency)
         block *= 2;
         waves = ceil(waves / 2);
     }
     if (block < f.block) block = f.block;
-    // (loaders: the rows that eight warps turn)
-    const double turned = (p.loose & linear::kLooseW ? 350 : 0) + (p.loose & linear::kLooseX ? 100 + 2.0 * p.cols : 0);
-    if (block < turned) block = turned;
     const double finish = f.finish + f.column * p.cols, blocks = p.per < p.kblocks ? p.per : p.kblocks;
     const double clocks = waves * (blocks * block + finish * (p.accumulators == 1 ? 1 : f.shown)) + (p.accumulators == 1 ? 0 : finish);
     const double weight = p.bits ? N * (K / 8.0) : 2.0 * N * K;
@@ -129,11 +125,11 @@ double plan_time(const linear::Plan& p, int M, int N, int K, int sms) {
 }
 
 // The plan that takes least.
-linear::Plan make_plan(int M, int N, int K, bool bits, int loose, int sms) {
+linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
     linear::Plan best = {};
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
-    for (int shape = 0; shape < (bits || loose ? 4 : 5); shape++) {               // K in 1, 2, 4, 8; pairs of CTAs
+    for (int shape = 0; shape < (bits ? 4 : 5); shape++) {               // K in 1, 2, 4, 8; pairs of CTAs
         const bool pair = shape == 4;
         const int splits = pair ? 1 : 1 << shape;
         if (g_linear_splits && g_linear_splits != (pair ? -2 : splits)) continue;
@@ -143,8 +139,7 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int loose, int sms) {
             linear::Plan p = {};
             p.bits = bits;
             p.form = pair ? linear::PAIR : splits > 1 ? linear::SPLIT : linear::ALONE;
-            if (((bits && splits > 1) || loose) && cols > 128) continue;
-            p.loose = loose;
+            if (bits && splits > 1 && cols > 128) continue;
             p.cols = cols;
             p.splits = splits;
             p.tiles_m = (M + cols - 1) / cols;
@@ -162,7 +157,7 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int loose, int sms) {
             p.columns = 32;
             while (p.columns < p.accumulators * cols + 32 * p.ring) p.columns *= 2;
             // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
-            const size_t room = (p.form == linear::SPLIT && !loose ? 113 : 227) * 1024;
+            const size_t room = (p.form == linear::SPLIT ? 113 : 227) * 1024;
             for (p.stages = linear::kMaxStages; p.stages > 2 && linear::smem_bytes(p) > room; p.stages--) {}
             const double t = plan_time(p, M, N, K, sms);
             if (t < least) { least = t; best = p; }
@@ -172,13 +167,12 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int loose, int sms) {
 }
 
 // (The last plans of this thread: the search takes a microsecond.)
-const linear::Plan& plan_linear(int M, int N, int K, bool bits, int loose, int sms) {
-    struct Kept { int M, N, K, kind, sms, cols, splits; linear::Plan plan; };
+const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
+    struct Kept { int M, N, K, bits, sms, cols, splits; linear::Plan plan; };
     static thread_local Kept kept[64];
-    const int kind = bits + 2 * loose;
-    Kept& k = kept[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 2246822519u ^ (unsigned)kind) >> 7 & 63];
-    if (k.M != M || k.N != N || k.K != K || k.kind != kind || k.sms != sms || k.cols != g_linear_cols || k.splits != g_linear_splits)
-        k = Kept{M, N, K, kind, sms, g_linear_cols, g_linear_splits, make_plan(M, N, K, bits, loose, sms)};
+    Kept& k = kept[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 2246822519u ^ (unsigned)bits) >> 7 & 63];
+    if (k.M != M || k.N != N || k.K != K || k.bits != (int)bits || k.sms != sms || k.cols != g_linear_cols || k.splits != g_linear_splits)
+        k = Kept{M, N, K, (int)bits, sms, g_linear_cols, g_linear_splits, make_plan(M, N, K, bits, sms)};
     return k.plan;
 }
 
@@ -187,22 +181,7 @@ const linear::Plan& plan_linear(int M, int N, int K, bool bits, int loose, int s
 bool small_pays(int M, int N, int K, int sms) {
     if (M > 128 || g_linear_cols || g_linear_splits) return false;
     const double us = 2.8 + (double)((M + 7) / 8) * N * K / 6.5e6;
-    return us < plan_time(plan_linear(M, N, K, true, 0, sms), M, N, K, sms);
-}
-
-// Operands that tensor copies cannot read
-int loose_operands(const void* x, long long ldx, int M, const void* W, long long ldw, int N) {
-    return (rows_fit(x, ldx, M) ? 0 : linear::kLooseX) | (!W || rows_fit(W, ldw, N) ? 0 : linear::kLooseW);
-}
-int g_linear_copy = 0;                                   // tcbnn_set_linear_copy: 0 = from the times, 1 = copied, 2 = turned
-// Whether such operands are copied to rows that tensor copies can read (a launch of 2.5 us, and three times their bytes), or turned by
-// the product's own loaders.
-bool copy_pays(int M, int N, int K, bool bits, int loose, int sms) {
-    if (!loose) return false;
-    if (g_linear_copy) return g_linear_copy == 1;
-    const linear::Plan own = plan_linear(M, N, K, bits, loose, sms), copied = plan_linear(M, N, K, bits, 0, sms);
-    const double bytes = 2.0 * K * ((loose & linear::kLooseX ? M : 0) + (loose & linear::kLooseW ? N : 0));
-    return !own.cols || (copied.cols && plan_time(copied, M, N, K, sms) + 2.5 + 3 * bytes / 4.5e6 < plan_time(own, M, N, K, sms));
+    return us < plan_time(plan_linear(M, N, K, true, sms), M, N, K, sms);
 }
 
 int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int width, int rows, long long pitch_bytes, int box_x, int box_y,
@@ -220,10 +199,9 @@ int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int
 int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const CUtensorMap& map_w, const CUtensorMap& map_x, cudaStream_t st) {
     using namespace linear;
     using Kernel = void (*)(Args, Plan, int*, CUtensorMap, CUtensorMap);
-    static const struct { bool bits; int form; bool loose; Kernel kernel; } of[] = {
-        {false, ALONE, false, k_linear<false, ALONE, false>}, {false, SPLIT, false, k_linear<false, SPLIT, false>}, {false, PAIR, false, k_linear<false, PAIR, false>},
-        {true, ALONE, false, k_linear<true, ALONE, false>},   {true, SPLIT, false, k_linear<true, SPLIT, false>},   {false, ALONE, true, k_linear<false, ALONE, true>},
-        {false, SPLIT, true, k_linear<false, SPLIT, true>},   {true, ALONE, true, k_linear<true, ALONE, true>},     {true, SPLIT, true, k_linear<true, SPLIT, true>}};
+    static const struct { bool bits; int form; Kernel kernel; } of[] = {
+        {false, ALONE, k_linear<false, ALONE>}, {false, SPLIT, k_linear<false, SPLIT>}, {false, PAIR, k_linear<false, PAIR>},
+        {true, ALONE, k_linear<true, ALONE>}, {true, SPLIT, k_linear<true, SPLIT>}};
     static bool done[64];
     static int* status_of[64];
     int dev = 0;
@@ -235,12 +213,12 @@ int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const C
             return e != cudaSuccess ? e : cudaGetSymbolAddress((void**)&status_of[dev & 63], g_linear_status);
         })) return 1;
     int i = 0;
-    while (of[i].bits != (bool)p.bits || of[i].form != p.form || of[i].loose != (p.loose != 0)) i++;
+    while (of[i].bits != (bool)p.bits || of[i].form != p.form) i++;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const int team = p.form == PAIR ? 2 : p.splits;
     const long long teams = p.form == SPLIT || tiles < sms / team ? tiles : sms / team;
-    const cudaError_t e = launch_dependent_cluster(of[i].kernel, (unsigned)(teams * team), team > 1 ? team : 0, threads_of(p.bits, p.loose), smem_bytes(p), st, a, p,
-                                                   status_of[dev & 63], map_w, map_x);
+    const cudaError_t e = launch_dependent_cluster(of[i].kernel, (unsigned)(teams * team), team > 1 ? team : 0, p.bits ? kThreadsBits : kThreadsDense, smem_bytes(p), st,
+                                                   a, p, status_of[dev & 63], map_w, map_x);
     if (e != cudaSuccess) return fail("linear: %s", cudaGetErrorString(e));
     return 0;
 }
@@ -288,12 +266,10 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     int sms;
     if (sm_count(&sms)) return 1;
     if (bits && small_pays(a.M, a.N, a.K, sms)) return run_bit_linear_small(a, sms, st);
-    int loose = loose_operands(a.x, a.ldx, a.M, bits ? nullptr : a.W, a.ldw, a.N);
-    if (copy_pays(a.M, a.N, a.K, bits, loose, sms)) {
-        const size_t need = tcbnn_linear_workspace_bytes(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
+    const size_t need = tcbnn_linear_workspace_bytes(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
+    if (need) {
         if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
             return fail("%s: these operands need %zu bytes of workspace, 256-byte aligned", what, need);
-        loose = 0;
         char* room = (char*)workspace;
         linear::Rows moved[2] = {};
         long long units = 0;
@@ -310,15 +286,13 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
         const cudaError_t e = launch_dependent(k_repack, (unsigned)(blocks < 16LL * sms ? blocks : 16LL * sms), 256, 0, st, moved[0], moved[1], a.K);
         if (e != cudaSuccess) return fail("%s: %s", what, cudaGetErrorString(e));
     }
-    const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, loose, sms);
+    const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, sms);
     if (!p.cols) return fail("%s: the forced plan does not exist for these operands", what);
     const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    CUtensorMap map_w = {}, map_x = {};
-    if (!(loose & linear::kLooseX) &&
-        linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, linear::own_cols(p), CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
-    if (!(loose & linear::kLooseW) &&
-        (bits ? linear_map(&map_w, a.W, CU_TENSOR_MAP_DATA_TYPE_UINT32, (a.K + 31) / 32, a.N, a.ldw * 4, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B)
-              : linear_map(&map_w, a.W, type, a.K, a.N, a.ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B))) return 1;
+    CUtensorMap map_w, map_x;
+    if (linear_map(&map_x, a.x, type, a.K, a.M, a.ldx * 2, 64, linear::own_cols(p), CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
+    if (bits ? linear_map(&map_w, a.W, CU_TENSOR_MAP_DATA_TYPE_UINT32, (a.K + 31) / 32, a.N, a.ldw * 4, 16, 128, CU_TENSOR_MAP_SWIZZLE_64B)
+             : linear_map(&map_w, a.W, type, a.K, a.N, a.ldw * 2, 64, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return 1;
     return launch_linear(a, p, sms, map_w, map_x, st);
 }
 
@@ -359,10 +333,8 @@ extern "C" {
 
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw) {
     int sms;
-    if (M < 1 || N < 1 || K < 1) return 0;
-    const int loose = loose_operands(x, ldx, M, W, ldw, N);
-    if (!loose || sm_count(&sms) || (!W && small_pays(M, N, K, sms)) || !copy_pays(M, N, K, !W, loose, sms)) return 0;
-    return (loose & linear::kLooseX ? packed_bytes(M, K) : 0) + (loose & linear::kLooseW ? packed_bytes(N, K) : 0);
+    if (M < 1 || N < 1 || K < 1 || (!W && !sm_count(&sms) && small_pays(M, N, K, sms))) return 0;
+    return (rows_fit(x, ldx, M) ? 0 : packed_bytes(M, K)) + (!W || rows_fit(W, ldw, N) ? 0 : packed_bytes(N, K));
 }
 
 int tcbnn_linear(const void* x, const void* W, const void* bias, const void* residual, void* out, int M, int N, int K, long long ldx,
@@ -377,12 +349,6 @@ int tcbnn_set_linear_plan(int cols, int splits) {
         return fail("set_linear_plan: cols is 0 or a multiple of 16 up to 256, splits is 0, 1, 2, 4 or 8, or -2 (pairs; cols a multiple of 32)");
     g_linear_cols = cols;
     g_linear_splits = splits;
-    return 0;
-}
-
-int tcbnn_set_linear_copy(int copy) {
-    if (copy < 0 || copy > 2) return fail("set_linear_copy: 0 = automatic, 1 = copied, 2 = turned by the product's loaders");
-    g_linear_copy = copy;
     return 0;
 }
 

@@ -9,8 +9,6 @@
 //   warp  9     loader x  : tensor copies of `cols` rows x 64
 //   warp  10    MMA       : converged, elected lane; four MMAs of K = 16 per 64
 //   warps 12-15 expanders : (packed) signs to +-1 in tensor memory, where the MMA reads its W operand
-//   last 8      (LOOSE) loaders of operands whose rows do not all start on 16 bytes, which tensor copies cannot read: a warp a row,
-//                         a word a lane, turned by two bytes where the row starts on an odd element
 //
 // Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.  Packed weights cost a
 // sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port either.
@@ -26,8 +24,7 @@
 namespace tcbnn {
 namespace linear {
 
-__host__ __device__ constexpr int threads_of(bool bits, bool loose) { return ((bits ? 16 : loose ? 12 : 11) + (loose ? 8 : 0)) * 32; }
-constexpr int kLooseX = 1, kLooseW = 2;
+constexpr int kThreadsDense = 11 * 32, kThreadsBits = 16 * 32;
 constexpr int kMaxCols = 256, kMaxStages = 12, kMaxRing = 8, kRawStages = 3;
 constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 rows of 64 elements, of 512 bits
 
@@ -40,7 +37,6 @@ struct Plan {
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
     int columns;                                       // of tensor memory
-    int loose;                                         // kLooseX, kLooseW: operands that tensor copies cannot read
 };
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
@@ -302,47 +298,12 @@ struct Output16 {
     }
 };
 
-// Sixteen rows of 64 elements, as words: lane i has word i of every row, and lane r the word behind row r's 32nd.
-struct LooseRows {
-    uint32_t w[16], behind;
-    __device__ __forceinline__ void ask(const uint16_t* base, long long ld, int row0, int rows, int k0, int K) {
-        const int lane = threadIdx.x & 31, left = K - k0;
-        behind = 0;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            w[r] = 0;
-            if (row0 + r >= rows) continue;
-            const uintptr_t p = reinterpret_cast<uintptr_t>(base + (row0 + r) * ld + k0);
-            const int odd = (int)(p >> 1) & 1;
-            // (words that hold an element of the row; the other half of its first and last may be its neighbours')
-            if (2 * lane - odd < left) w[r] = ld_dep(reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3) + lane);
-            if (lane == r && odd && left >= 64) behind = ld_dep(reinterpret_cast<const uint32_t*>(p & ~(uintptr_t)3) + 32);
-        }
-    }
-    // into a stage's rows of 128 bytes, their 16-byte pieces turned by the row (the MMA's 128-byte swizzle)
-    __device__ __forceinline__ void put(uint32_t tile, const uint16_t* base, long long ld, int row0, int held, int k0, int K) const {
-        const int lane = threadIdx.x & 31, left = K - k0 - 2 * lane;       // elements of the lane's two that exist
-        const uint32_t keep = left >= 2 ? 0xFFFFFFFFu : left == 1 ? 0xFFFFu : 0u;
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-            if (row0 + r >= held) break;
-            const uint32_t odd = (uint32_t)(reinterpret_cast<uintptr_t>(base + (row0 + r) * ld + k0) >> 1) & 1u;
-            uint32_t next = __shfl_down_sync(0xffffffffu, w[r], 1);
-            const uint32_t last = __shfl_sync(0xffffffffu, behind, r);
-            if (lane == 31) next = last;
-            const uint32_t v = __funnelshift_r(w[r], next, 16 * odd) & keep;
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(tile + (row0 + r) * 128 + (((lane >> 2) ^ ((row0 + r) & 7)) << 4) + (lane & 3) * 4), "r"(v) : "memory");
-        }
-    }
-};
-
-template <bool BITS, int FORM, bool LOOSE>
+template <bool BITS, int FORM>
 __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUtensorMap* map_w, const CUtensorMap* map_x, int* status,
                                          unsigned char* smem0) {
     using namespace umma;
     unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem0) + 1023) & ~(uintptr_t)1023);
     constexpr bool CLUSTER = FORM == SPLIT, PAIRED = FORM == PAIR;
-    static_assert(!LOOSE || !PAIRED, "loose operands are for one CTA");
     static_assert(!BITS || !PAIRED, "no pairs with packed weights: they were no faster");
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t nctas = CLUSTER ? [] { uint32_t n; asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n)); return n; }() : 1u;
@@ -379,11 +340,11 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     };
 
     if (warp == 8 && lane == 0) {
-        if (!LOOSE || !(p.loose & kLooseW)) asm volatile("prefetch.tensormap [%0];" ::"l"(map_w) : "memory");
-        if (!LOOSE || !(p.loose & kLooseX)) asm volatile("prefetch.tensormap [%0];" ::"l"(map_x) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map_x) : "memory");
     }
     if (tid == 0) {
-        for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), (BITS ? 1 : 2) + (LOOSE ? 8 - __popc(p.loose) : 0)); mbar_init(EMPTY(s), 1); }
+        for (int s = 0; s < kMaxStages; s++) { mbar_init(FULL(s), BITS ? 1 : 2); mbar_init(EMPTY(s), 1); }
         for (int s = 0; s < kMaxRing; s++) { mbar_init(RFULL(s), 4); mbar_init(REMPTY(s), 1); }
         for (int s = 0; s < kRawStages; s++) { mbar_init(RAWFULL(s), 1); mbar_init(RAWEMPTY(s), 4); }
         for (int b = 0; b < 2; b++) { mbar_init(SFULL(b), 1); mbar_init(SEMPTY(b), PAIRED ? 16 : 8); }
@@ -412,8 +373,8 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
 
     if (warp == 8 || warp == 9) {
         // =============================== loaders ============================================
-        const bool isw = warp == 8, loose = LOOSE && (p.loose & (isw ? kLooseW : kLooseX));
-        if (lane == 0 && nkb > 0 && !loose) {
+        if (lane == 0 && nkb > 0) {
+            const bool isw = warp == 8;
             const int step = BITS && isw ? 8 : 1, slots = BITS && isw ? kRawStages : p.stages;
             int s = 0, issued = 0;
             uint32_t ph = 0;
@@ -495,50 +456,6 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                 mma_commit(DRAIN);
             for (int i = 0; i < (1 << 20); i++)
                 if (PAIRED ? mbar_test_cluster(DRAIN, 0) : mbar_try_wait(DRAIN, 0)) break;
-        }
-        __syncwarp();
-    } else if (LOOSE && warp >= (BITS ? 16 : 12)) {
-        // =============================== loaders of loose operands ==========================
-        const int row0 = (warp - (BITS ? 16 : 12)) * 16;
-        const uint16_t* of_x = reinterpret_cast<const uint16_t*>(a.x);
-        const uint16_t* of_w = reinterpret_cast<const uint16_t*>(a.W);
-        const bool lx = p.loose & kLooseX, lw = !BITS && (p.loose & kLooseW);
-        int s = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        LooseRows x[2], w[2];
-        const int steps = nkb > 0 ? (ntiles - t_first + t_step - 1) / t_step * nkb : 0;
-        auto at = [&](int i, int& tm, int& tn, int& k0) {            // position i of the CTA's sequence of (tile, block of K)
-            const int j = i / nkb;
-            tile(t_first + j * t_step, tm, tn);
-            k0 = (kb0 + i - j * nkb) * 64;
-        };
-        auto ask = [&](int i, LooseRows& xr, LooseRows& wr) {
-            int tm, tn, k0;
-            at(i, tm, tn, k0);
-            if (lx && row0 < own) xr.ask(of_x + (long long)tm * p.cols * a.ldx, a.ldx, row0, min(own, a.M - tm * p.cols), k0, a.K);
-            if (lw) wr.ask(of_w + (long long)tn * 128 * a.ldw, a.ldw, row0, min(128, a.N - tn * 128), k0, a.K);
-        };
-        auto put = [&](int i, const LooseRows& xr, const LooseRows& wr) {
-            int tm, tn, k0;
-            at(i, tm, tn, k0);
-            ok = wait(EMPTY(s), ph ^ 1);
-            if (!ok) return;
-            const uint32_t dst = smem_u32(smem) + s * stage;
-            if (lx && row0 < own) xr.put(dst + (BITS ? 0u : kWStage), of_x + (long long)tm * p.cols * a.ldx, a.ldx, row0, own, k0, a.K);
-            if (lw) wr.put(dst, of_w + (long long)tn * 128 * a.ldw, a.ldw, row0, 128, k0, a.K);
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(FULL(s));
-            if (++s == p.stages) { s = 0; ph ^= 1; }
-        };
-        if (steps > 0) ask(0, x[0], w[0]);
-        for (int i = 0; i < steps && ok; i += 2) {       // (the next block is under way while one is stored)
-            if (i + 1 < steps) ask(i + 1, x[1], w[1]);
-            put(i, x[0], w[0]);
-            if (i + 1 >= steps || !ok) break;
-            if (i + 2 < steps) ask(i + 2, x[0], w[0]);
-            put(i + 1, x[1], w[1]);
         }
         __syncwarp();
     } else if (BITS && warp >= 12) {

@@ -278,12 +278,6 @@ def set_linear_plan(cols=0, splits=0):
     _l.call("tcbnn_set_linear_plan", int(cols), int(splits))
 
 
-def set_linear_copy(copy=0):
-    """Operands of linear() and bit_linear() whose rows do not all start on 16 bytes: 1 = copied first, 2 = turned by the
-    product's own loaders, 0 = automatic."""
-    _l.call("tcbnn_set_linear_copy", int(copy))
-
-
 def linear_status():
     s = C.c_int(0)
     _l.call("tcbnn_linear_status", C.byref(s))

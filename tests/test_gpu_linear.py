@@ -182,49 +182,13 @@ def test_rows_apart_and_what_lies_between_them(cuda, bits, dtype, M, N, K, pad):
         assert (rbuf[mask] == 5.0).all()
 
 
-@pytest.mark.parametrize("copy", [1, 2])
-@pytest.mark.parametrize("bits", [False, True])
-@pytest.mark.parametrize("cols,splits", [(0, 0), (16, 1), (64, 2), (128, 1), (96, 4)])
-@pytest.mark.parametrize("M,N,K,x_shift,w_shift", [(1, 300, 65, 0, 0), (9, 129, 1001, 1, 0), (200, 700, 130, 0, 3), (333, 1000, 2049, 2, 1), (2000, 1500, 63, 7, 7),
-                                                   (64, 4096, 64, 0, 1), (64, 4096, 128, 1, 0)])
-def test_loose_rows(cuda, copy, bits, cols, splits, M, N, K, x_shift, w_shift):
-    """Rows that start on any element, copied or turned by the product's loaders, one operand or both, under forced plans too."""
-    x0, w0, scale, sums = case(bits, M, N, K, FP16, cuda)
-    xb = torch.full((M, K + x_shift + 1), math.nan, dtype=FP16, device=cuda)
-    x, w = xb[:, x_shift:x_shift + K], w0
-    x.copy_(x0)
-    if not bits:
-        wb = torch.full((N, K + w_shift), math.nan, dtype=FP16, device=cuda)
-        w = wb[:, w_shift:]
-        w.copy_(w0)
-    ops.set_linear_plan(cols, splits)
-    ops.set_linear_copy(copy)
-    try:
-        got = product(bits, x, w, scale, out_dtype=FP32)
-        assert ops.linear_status() == 0
-    finally:
-        ops.set_linear_plan()
-        ops.set_linear_copy()
-    assert torch.equal(got.double(), sums)
-
-
 @pytest.mark.parametrize("bits", [False, True])
 @pytest.mark.parametrize("M,N,K", [(3, 50, 77), (500, 600, 333)])
 def test_workspaces(cuda, bits, M, N, K):
     """A workspace of one's own, for operands that need one; too small ones and none are refused by the library."""
     x, w, scale, sums = case(bits, M, N, K, BF16, cuda)
-    assert bits and M == 3 or ops.linear_workspace(x, w) is None         # (small ones are turned)
-    ops.set_linear_copy(1)
-    try:
-        ws = ops.linear_workspace(x, w)
-        assert (ws is None) == (bits and M == 3)       # (few rows of packed weights are read where they lie)
-        check_workspace(cuda, bits, x, w, scale, sums, ws)
-    finally:
-        ops.set_linear_copy()
-
-
-def check_workspace(cuda, bits, x, w, scale, sums, ws):
-    M, K = x.shape
+    ws = ops.linear_workspace(x, w)
+    assert (ws is None) == (bits and M == 3)           # (few rows of packed weights are read where they lie)
     assert torch.equal(product(bits, x, w, scale, out_dtype=FP32, workspace=ws).double(), sums)
     aligned = torch.zeros((M, 80 if K == 77 else 336), dtype=BF16, device=cuda)
     assert ops.linear_workspace(aligned, w if bits else aligned) is None
