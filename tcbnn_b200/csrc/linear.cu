@@ -3,7 +3,7 @@
 #include <cmath>
 #include "host.cuh"
 #include "bnn_layers.cuh"
-#include "bit_linear_small.cuh"
+#include "linear_small.cuh"
 #include "log_probs.cuh"
 
 using namespace tcbnn;
@@ -22,6 +22,11 @@ template <int RT, bool BF>
 __global__ void __launch_bounds__(32 * linear::kSmallWarps, 1) k_bit_linear_small(linear::Args a) {
     extern __shared__ __align__(16) float bit_linear_sums[];
     linear::bit_linear_small<RT, BF>(a, bit_linear_sums);
+}
+template <bool BF, bool WIDE>
+__global__ void __launch_bounds__(32 * linear::kDenseWarps, 2) k_linear_small(linear::Args a) {
+    __shared__ float sums[linear::kDenseWarps * 8 * 20];
+    linear::linear_small<BF, WIDE>(a, sums);
 }
 __global__ void __launch_bounds__(256) k_repack(linear::Rows x, linear::Rows w, int K) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -95,6 +100,9 @@ int check_linear(const char* what, const linear::Args& a, bool bits) {
 // Operands that tensor copies can read: rows that start on multiples of 16 bytes (less than 2^40 bytes apart)
 bool rows_fit(const void* p, long long ld, int rows) {
     return ((uintptr_t)p & 15) == 0 && (rows == 1 || ((ld & 7) == 0 && ld < (1LL << 39)));
+}
+double bytes_to_copy(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw) {
+    return 2.0 * K * ((rows_fit(x, ldx, M) ? 0 : M) + (!W || rows_fit(W, ldw, N) ? 0 : N));
 }
 size_t packed_bytes(int rows, int K) { return ((size_t)rows * ((K + 7) & ~7) * 2 + 255) & ~(size_t)255; }
 
@@ -176,12 +184,38 @@ const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
     return k.plan;
 }
 
-// Packed weights and few rows: whether the kernel on warp-level MMAs is the faster one.  It takes 2.8 us and what its expansions take,
-// 6.5e6 weights a us for every eight rows (8192 x 8192 for 24 rows 34 us, 4096 x 4096 for 32 13, for one 4.1; the other kernel 17.5, 9.5, 8.6).
-bool small_pays(int M, int N, int K, int sms) {
+// What the launch that copies operands in front of the product takes
+double copy_time(double bytes) { return bytes > 0 ? 2.3 + bytes * 0.36e-6 : 0; }
+// Few rows: whether the kernels on warp-level MMAs are the faster ones.  Packed weights: 2.8 us and 6.5e6 expansions a us for every eight
+// rows (8192 x 8192 for 24 rows 34 us, 4096 x 4096 for 32 13, for one 4.1; the other kernel 17.5, 9.5, 8.6).  Dense ones: 2.1 us
+// and their bytes at 5.7 TB/s for every eight rows, or a warp's pieces one after another (4096 x 4096 for one row 8.3 us, 512 x 512 for 64
+// 2.4, 4096 x 9216 for 16 25; the other kernel 9.4, 4.4, 16.4); rows that start on any element at 2.6 TB/s (1 x 4097 -> 4096 15.0,
+// 32 x 1001 -> 1000 5.1, copied first 22.5, 7.8).  copied: bytes that the other kernel needs copied.
+bool small_pays(int M, int N, int K, bool bits, double copied, int sms) {
     if (M > 128 || g_linear_cols || g_linear_splits) return false;
-    const double us = 2.8 + (double)((M + 7) / 8) * N * K / 6.5e6;
-    return us < plan_time(plan_linear(M, N, K, true, sms), M, N, K, sms);
+    const double groups = (M + 7) / 8, weights = (double)N * K;
+    double us = 2.8 + groups * weights / 6.5e6;
+    if (!bits) {
+        const double bytes = groups * 2 * weights * (copied > 0 ? 0.39e-6 : 0.175e-6), pieces = ceil(ceil(K / 128.0) / 8) * (copied > 0 ? 0.8 : 0.55);
+        us = 2.1 + (bytes > pieces ? bytes : pieces);
+    }
+    return us < plan_time(plan_linear(M, N, K, bits, sms), M, N, K, sms) + copy_time(copied);
+}
+
+// A launch of few rows' kernel: outputs x rows
+int launch_small(void (*kernel)(linear::Args), const linear::Args& a, int outputs, int threads, size_t smem, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((a.N + outputs - 1) / outputs, (a.M + 7) / 8);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+    return e != cudaSuccess ? fail("linear: %s", cudaGetErrorString(e)) : 0;
 }
 
 int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int width, int rows, long long pitch_bytes, int box_x, int box_y,
@@ -245,19 +279,15 @@ int run_bit_linear_small(const linear::Args& a, int sms, cudaStream_t st) {
     const long long blocks = (long long)((a.N + 16 * rt - 1) / (16 * rt)) * ((a.M + 7) / 8);
     int warps = blocks <= sms ? kSmallWarps : kSmallWarps / 2;
     if (warps > pieces) warps = pieces;
-    const dim3 grid((a.N + 16 * rt - 1) / (16 * rt), (a.M + 7) / 8);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(32 * warps);
-    cfg.dynamicSmemBytes = small_bytes(rt, warps);
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, a.type == TCBNN_BF16 ? of[i].bf16 : of[i].fp16, a);
-    return e != cudaSuccess ? fail("bit_linear: %s", cudaGetErrorString(e)) : 0;
+    return launch_small(a.type == TCBNN_BF16 ? of[i].bf16 : of[i].fp16, a, 16 * rt, 32 * warps, small_bytes(rt, warps), st);
+}
+
+int run_linear_small(const linear::Args& a, cudaStream_t st) {
+    using namespace linear;
+    const bool wide = rows_fit(a.x, a.ldx, a.M) && rows_fit(a.W, a.ldw, a.N);
+    auto kernel = a.type == TCBNN_BF16 ? wide ? k_linear_small<true, true> : k_linear_small<true, false>
+                                       : wide ? k_linear_small<false, true> : k_linear_small<false, false>;
+    return launch_small(kernel, a, 16, 32 * kDenseWarps, 0, st);
 }
 
 int run_linear(const char* what, linear::Args a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {
@@ -265,7 +295,8 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
     if (a.M == 0) return 0;
     int sms;
     if (sm_count(&sms)) return 1;
-    if (bits && small_pays(a.M, a.N, a.K, sms)) return run_bit_linear_small(a, sms, st);
+    const double copied = bytes_to_copy(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
+    if (small_pays(a.M, a.N, a.K, bits, copied, sms)) return bits ? run_bit_linear_small(a, sms, st) : run_linear_small(a, st);
     const size_t need = tcbnn_linear_workspace_bytes(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
     if (need) {
         if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
@@ -333,7 +364,9 @@ extern "C" {
 
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw) {
     int sms;
-    if (M < 1 || N < 1 || K < 1 || (!W && !sm_count(&sms) && small_pays(M, N, K, sms))) return 0;
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const double copied = bytes_to_copy(x, W, M, N, K, ldx, ldw);
+    if (copied == 0 || (!sm_count(&sms) && small_pays(M, N, K, !W, copied, sms))) return 0;
     return (rows_fit(x, ldx, M) ? 0 : packed_bytes(M, K)) + (!W || rows_fit(W, ldw, N) ? 0 : packed_bytes(N, K));
 }
 

@@ -62,7 +62,7 @@ def product(bits, x, w, scale, *args, **kw):
 SHAPES = [(1, 1, 1), (1, 3, 7), (1, 128, 16), (1, 4096, 4096), (2, 130, 70), (3, 64, 8), (5, 1000, 2049), (8, 4096, 136), (15, 250, 512),
           (16, 129, 64), (17, 300, 1025), (31, 77, 3000), (33, 1, 65), (64, 512, 576), (65, 2000, 128), (100, 10, 9000), (129, 257, 130),
           (192, 128, 4100), (193, 1000, 333), (255, 256, 257), (300, 1024, 4096), (513, 640, 200), (777, 4096, 1216), (1000, 384, 96),
-          (2049, 1111, 1000), (4096, 2048, 512), (1, 20000, 24), (2, 64, 16384), (40, 8192, 16384)]
+          (8, 64, 16384), (12, 4096, 4097), (33, 515, 259), (64, 1000, 1001), (120, 16, 31), (2049, 1111, 1000), (4096, 2048, 512), (1, 20000, 24), (2, 64, 16384), (40, 8192, 16384)]
 
 
 @pytest.mark.parametrize("bits", [False, True])
@@ -188,7 +188,7 @@ def test_workspaces(cuda, bits, M, N, K):
     """A workspace of one's own, for operands that need one; too small ones and none are refused by the library."""
     x, w, scale, sums = case(bits, M, N, K, BF16, cuda)
     ws = ops.linear_workspace(x, w)
-    assert (ws is None) == (bits and M == 3)           # (few rows of packed weights are read where they lie)
+    assert (ws is None) == (M == 3)                    # (few rows are read where they lie)
     assert torch.equal(product(bits, x, w, scale, out_dtype=FP32, workspace=ws).double(), sums)
     aligned = torch.zeros((M, 80 if K == 77 else 336), dtype=BF16, device=cuda)
     assert ops.linear_workspace(aligned, w if bits else aligned) is None
