@@ -403,7 +403,8 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
 #define TCBNN_GELU 2
 #define TCBNN_GELU_TANH 3
 #define TCBNN_SILU 4
-/* out[m][n] = act(sum_k x[m][k] * W[n][k] + bias[n]) + residual[m][n], for M >= 0 rows of x and N, K >= 1.
+/* out[m][n] = act(sum_k x[m][k] * W[n][k] + bias[n]) + residual[m][n], for M >= 0 rows of x and N, K >= 1 (M, N up to 2^30, K
+ * up to 2^24).
  * x [M][ldx] and W [N][ldw] are of `type` (fp16 or bf16), bias [N] (or NULL) of that type or fp32 (bias_type), residual [M][ldr]
  * (or NULL) and out [M][ldo] of `type` or fp32 (out_type).  Leading dimensions count elements; what lies between rows is neither
  * read nor written.  Sums, activation and residual are fp32, the result is rounded once.
@@ -428,7 +429,7 @@ int tcbnn_linear_status(int* status);
  * of up to 128 tokens; a forced plan also keeps few rows off the kernel on warp-level MMAs.  Calls without the forced plan fail.
  * Process-wide; for tests and measurements. */
 int tcbnn_set_linear_plan(int cols, int splits);
-/* Scores of M rows of V logits (fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
+/* Scores of M rows of V logits (V up to 2^30; fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
  *                                            0 for a negative target (a row without one), NaN for one past V - 1
  *   entropy[m]  = ln S - sum(e^d d) / S      or NULL

@@ -69,6 +69,10 @@ bool apart(const Block& a, const Block& b) {
 
 int check_linear(const char* what, const linear::Args& a, bool bits) {
     if (a.M < 0 || a.N < 1 || a.K < 1) return fail("%s: M >= 0, N and K >= 1", what);
+    // (the largest K keeps a tile's time far inside the waits' limits)
+    if (a.M > 1 << 30 || a.N > 1 << 30 || a.K > 1 << 24) return fail("%s: M and N up to 2^30, K up to 2^24", what);
+    const long long far = 1LL << 40;
+    if (a.ldx > far || a.ldw > far || a.ldo > far || (a.residual && a.ldr > far)) return fail("%s: leading dimensions up to 2^40", what);
     if (a.type != TCBNN_FP16 && a.type != TCBNN_BF16) return fail("%s: x is fp16 or bf16", what);
     if (a.out_type != a.type && a.out_type != TCBNN_FP32) return fail("%s: the result is of x's type or fp32", what);
     if (a.bias_type != a.type && a.bias_type != TCBNN_FP32) return fail("%s: the bias is of x's type or fp32", what);
@@ -413,9 +417,10 @@ int tcbnn_set_log_probs_plan(int warps, int ctas) {
 
 int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, const void* targets, int target_bytes, float temperature,
                     int top, float* logp, float* entropy, int64_t* top_ids, float* top_logp, void* stream) {
-    if (M < 0 || V < 1) return fail("log_probs: M >= 0 and V >= 1");
+    if (M < 0 || V < 1 || V > 1 << 30) return fail("log_probs: M >= 0 and V >= 1, up to 2^30");
     if (type != TCBNN_FP32 && type != TCBNN_FP16 && type != TCBNN_BF16) return fail("log_probs: logits are fp32, fp16 or bf16");
     if (ld < V) return fail("log_probs: rows closer together than they are long");
+    if (ld > 1LL << 40) return fail("log_probs: ld up to 2^40");
     if (targets && target_bytes != 4 && target_bytes != 8) return fail("log_probs: targets are int32 or int64");
     if (!(temperature >= 1e-30f && temperature <= 1e30f)) return fail("log_probs: the temperature must be between 1e-30 and 1e30");
     if (top < 0 || top > scores::kMaxTop || top > V) return fail("log_probs: top must be between 0 and %d and at most V", scores::kMaxTop);

@@ -32,7 +32,7 @@ constexpr uint32_t kWStage = 128 * 128, kRawStage = 128 * 64;            // 128 
 constexpr uint32_t kTurnPitch = 80, kTurn = 32 * kTurnPitch;
 enum Form { ALONE = 0, SPLIT = 1, PAIR = 2 };
 struct Plan {
-    int bits, form, cols, splits;                            // tokens per tile (a multiple of 16), CTAs that share K
+    int bits, form, cols, splits;                      // tokens per tile (a multiple of 16), CTAs that share K
     int tiles_m, tiles_n, band;                        // tiles of tokens and of outputs; token tiles worked on together
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
@@ -571,6 +571,10 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     }
     tc_fence_before();
     if constexpr (CLUSTER) {
+        // Tensor memory goes back before the CTAs wait for one another: one that holds some and waits for a peer that waits for some
+        // on another SM, held by a kernel of another stream that does the same, could wait forever.
+        __syncthreads();
+        if (warp == 10) tmem_dealloc(tmem, p.columns);
         // One tile per cluster: every CTA finishes each nctas-th group of four columns.
         cluster_sync();
         if (warp < 8 && !*sAbort) {
@@ -595,11 +599,11 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         }
         cluster_sync();                                  // nobody reads this CTA's sums any more
     }
-    __syncthreads();
+    if constexpr (!CLUSTER) __syncthreads();
     if constexpr (PAIRED) {
         cluster_sync();                                  // nothing of the partner's reaches into this CTA any more
         if (warp == 10) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.columns) : "memory");
-    } else if (warp == 10) {
+    } else if (!CLUSTER && warp == 10) {
         tmem_dealloc(tmem, p.columns);
     }
 }

@@ -233,6 +233,8 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
         res_p, ldr = residual.data_ptr(), _rows("residual", residual, device, ot, N, M)
     x_p, w_p, ws, ws_bytes = x.data_ptr(), weight.data_ptr(), None, 0
     if workspace is not None:
+        if workspace.get_device() != device:
+            raise _l.TcbnnError(f"the workspace is on {workspace.device}, the current device is cuda:{device}")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif (x_p | 2 * ldx | (0 if bits else w_p | 2 * ldw)) & 15 and M:
         # (rows that do not all start on 16 bytes)

@@ -17,7 +17,9 @@ def product(name="tcbnn_linear", scale=None, **kw):
     return rc, lib.load().tcbnn_last_error().decode()
 
 
-BAD = [(dict(N=0), "N and K"), (dict(K=0), "N and K"), (dict(M=-1), "M >= 0"), (dict(type=lib.FP32), "fp16 or bf16"), (dict(type=7), "fp16 or bf16"),
+BAD = [(dict(N=0), "N and K"), (dict(K=0), "N and K"), (dict(M=-1), "M >= 0"), (dict(M=(1 << 30) + 1), "2^30"),
+       (dict(N=(1 << 30) + 1, ldo=1 << 31, ldr=1 << 31), "2^30"), (dict(K=(1 << 24) + 1, ldx=1 << 25), "2^24"), (dict(ldo=(1 << 40) + 8), "2^40"),
+       (dict(type=lib.FP32), "fp16 or bf16"), (dict(type=7), "fp16 or bf16"),
        (dict(out_type=lib.FP16), "x's type or fp32"), (dict(bias_type=lib.FP16), "x's type or fp32"), (dict(activation=5), "activation"),
        (dict(activation=-1), "activation"), (dict(x=None), "null"), (dict(W=None), "null"), (dict(out=None), "null"), (dict(ldx=127), "closer"),
        (dict(ldo=63), "closer"), (dict(ldr=63), "closer"), (dict(x=X + 1), "aligned"), (dict(out=O + 1), "aligned"), (dict(residual=R + 1), "aligned"),
@@ -64,7 +66,7 @@ def scores(**kw):
 
 
 @pytest.mark.parametrize("kw,says", [
-    (dict(M=-1), "M >= 0"), (dict(V=0), "V >= 1"), (dict(type=3), "fp32, fp16 or bf16"), (dict(ld=99), "closer"), (dict(target_bytes=2), "int32 or int64"),
+    (dict(M=-1), "M >= 0"), (dict(V=0), "V >= 1"), (dict(V=(1 << 30) + 1, ld=1 << 31), "2^30"), (dict(ld=(1 << 40) + 1), "2^40"), (dict(type=3), "fp32, fp16 or bf16"), (dict(ld=99), "closer"), (dict(target_bytes=2), "int32 or int64"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(temperature=float("inf")), "temperature"),
     (dict(temperature=-1.0), "temperature"), (dict(top=33), "top"), (dict(top=-1), "top"), (dict(top=6, V=5, ld=5), "top"), (dict(logits=None), "null"),
     (dict(ids=None), "null"), (dict(top_logp=None), "null"), (dict(logp=None), "null"), (dict(logits=X + 2), "aligned"), (dict(targets=W + 4), "aligned"),
