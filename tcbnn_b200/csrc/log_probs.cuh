@@ -310,14 +310,22 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
     };
     // (-inf: no part in anything)
     const uint32_t fill = TYPE == linear::FP32 ? 0xFF800000u : TYPE == linear::BF16 ? 0xFF80FF80u : 0xFC00FC00u;
-    auto load = [&](uint4 (&v)[U], int i0) {
+    // of a thread, U vectors THREADS apart each: so many batches that every thread has in full, and one more that some have in part
+    const int i0 = v0 + tid, full = (v1 - v0) / (U * THREADS), batches = (v1 - v0 + U * THREADS - 1) / (U * THREADS);
+    const char* at_v = body + (long long)i0 * 16;
+    auto load = [&](uint4 (&v)[U], int b) {
+        if (b < full) {
 #pragma unroll
-        for (int u = 0; u < U; u++) v[u] = i0 + u * THREADS < v1 ? load16(body + (long long)(i0 + u * THREADS) * 16) : make_uint4(fill, fill, fill, fill);
+            for (int u = 0; u < U; u++) v[u] = load16(at_v + u * THREADS * 16);
+        } else if (b < batches) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                v[u] = i0 + (b * U + u) * THREADS < v1 ? load16(at_v + u * THREADS * 16) : make_uint4(fill, fill, fill, fill);
+        }
+        at_v += U * THREADS * 16;
     };
-
     uint4 cur[U], next[U];
-    int i0 = v0 + tid;
-    load(cur, i0);
+    load(cur, 0);
     // the ends: a thread each
     int at = -1;
     float end = -INFINITY;
@@ -330,9 +338,9 @@ __device__ __forceinline__ void row(const Args& a, Shared<NW>& s, long long r, u
         target = a.target_bytes == 8 ? reinterpret_cast<const long long*>(a.targets)[r] : reinterpret_cast<const int*>(a.targets)[r];
         if (target >= 0 && target < a.V) given = linear::load(base, target, TYPE);
     }
-    for (; i0 - lane < v1; i0 += U * THREADS) {        // (of the warp)
-        load(next, i0 + U * THREADS);
-        batch(cur);
+    for (int b = 0; b < batches; b++) {
+        load(next, b + 1);
+        if (b < full || i0 - lane + b * U * THREADS < v1) batch(cur);    // (of the warp)
 #pragma unroll
         for (int u = 0; u < U; u++) cur[u] = next[u];
     }
