@@ -10,13 +10,24 @@
 //   warp  10    MMA       : converged, elected lane; four MMAs of K = 16 per 64
 //   warps 12-15 expanders : (packed) signs to +-1 in tensor memory, where the MMA reads its W operand
 //
-// Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.  Packed weights cost a
-// sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port either.
+// Tensor copies fill rows and elements past the end with zeros, so no size needs a case of its own.
+//
+// Packed weights cost a sixteenth of the bytes, and expanded in tensor memory they take nothing of the shared-memory port, which rows
+// of x fill.  An MMA takes 100 clocks that way at least, whatever its columns, and a block of 64 of K 400 to 570 with what the
+// expanders wait for: few tokens are another kernel's (linear_small.cuh).  Expanded in shared memory instead, 475 clocks; two groups of
+// expanders, no faster at 256 columns (472 us against 466, below); blocks handed over in twos and fours, 420 clocks, but
+// 680 at 256 columns; pairs of SMs, 429 us against 410: all taken back.
 //
 // Where tiles of 128 x cols leave SMs idle, K is cut over a cluster's CTAs (SPLIT), whose sums meet in shared memory, in rank
 // order: the same result every time.  Where there are enough, pairs of SMs own tiles of 256 outputs (PAIR): each CTA holds its
 // 128 rows of W and half of the tokens' rows, the leader issues MMAs that read both (cta_group::2), so that rows of x
 // come from L2 and out of shared memory half as often.
+//
+// What bounds it: large products the GPU's power.  4096 x 16384 x 4096 over a second takes 400 us in pairs (1374 TFLOP/s, 1.3 GHz, 0.98 of
+// cuBLAS in the same minute), 437 without pairs, with gelu 408; packed weights 410, with gelu 456, as two sets of 256 columns do not fit
+// beside the expanded weights and half of an epilogue shows.  In a burst 350 (0.95 of the measured GEMM rate).  Few tokens: W's way from
+// memory, 16 x 9216 -> 4096 16.2 us for 75 MB (0.72 of the copy rate).  Between them a CTA's bytes from L2, 72 per clock, and
+// set-up and epilogue, 3 us of a launch.
 #pragma once
 #include "bconv_umma_pre.cuh"
 #include "linear.cuh"

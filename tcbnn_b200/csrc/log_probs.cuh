@@ -18,8 +18,13 @@
 // 83 without alternatives at 4096 x 50001.)  Where the list overflows -- more ties than it holds -- the row is read again, the
 // list cut to its best `top` as often as it fills.
 //
-// A warp, 8 of them share a row, or the CTAs of a cluster, whose parts meet in the first one's shared memory.
-// Bound: HBM; 16-bit logits at 6.46 TB/s are 3.2e12 exponentials a second, 0.7 of what the units for them do.
+// One to eight warps share a row, or the CTAs of a cluster, whose parts meet in the first one's shared memory.  (A thread's share depends
+// on where the row starts modulo 16 bytes, and with it the order of the sums, not the values that are compared.)
+//
+// What bounds it: long rows the issue slots, 2.75 instructions a clock of 4 while 0.55 of the special-function units' slots and 0.70 of
+// HBM's copy rate are used (4096 x 50001 bf16, 410 MB: 90.5 us with eight alternatives, 75.0 without); few or short rows the chain
+// load, sums, bound, second look, sort (8 x 1000 fp32 4.0 us, 1 x 131072 bf16 6.4, of which a launch is 2).  24 warps an SM instead of
+// 32, 107 us; 40 warps with 32 bytes a thread, 94.5; the row that follows fetched into L2 ahead, 97 to 127.
 #pragma once
 #include "linear.cuh"
 
