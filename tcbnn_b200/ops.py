@@ -264,8 +264,8 @@ def linear_workspace(x, weight):
 def linear(x, weight, bias=None, activation="none", residual=None, out=None, out_dtype=None, workspace=None):
     """act(x @ weight.T + bias) + residual, sums in fp32, rounded once (tcbnn_linear).
     x [M][K] and weight [N][K]: bf16 or fp16, rows contiguous, any distance apart; rows that start on multiples of 16 bytes are read
-    as they are, others copied first.  bias [N]: x's type or fp32.  residual [M][N] and out: x's type or fp32 (out_dtype); residual
-    may be out itself.  activation: "none", "relu", "gelu", "gelu_tanh" or "silu"."""
+    as they are, others copied first where there are many rows.  bias [N]: x's type or fp32.  residual [M][N] and out: x's type or
+    fp32 (out_dtype); residual may be out itself.  activation: "none", "relu", "gelu", "gelu_tanh" or "silu".  The result carries no gradient."""
     return _product(x, weight, None, bias, activation, residual, out, out_dtype, workspace, False)
 
 
@@ -295,7 +295,7 @@ def log_probs(logits, targets=None, top=0, temperature=1.0):
     """(logp [M], entropy [M], top_ids [M][top], top_logp [M][top]) of logits [M][V] (fp32, fp16 or bf16, rows contiguous, any
     distance apart) divided by `temperature` (tcbnn_log_probs).
     logp: of the given tokens targets [M] (int32 or int64), 0 where that is negative; None without targets.  top_ids (int64): the `top`
-    likeliest tokens (at most 32), equal ones in rising order; -1 behind the last token whose logit is not -inf."""
+    likeliest tokens (at most 32), equal ones in rising order; -1 behind the last token whose logit is not -inf.  No gradients."""
     device, code = _current_device(), _TYPES.get(logits.dtype)
     if code is None:
         raise _l.TcbnnError(f"logits are of torch.float32, torch.float16 or torch.bfloat16, not {logits.dtype}")

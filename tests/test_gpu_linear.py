@@ -7,6 +7,9 @@ result, which torch makes alike (to nearest even), so that outputs are compared 
 Activations: erff, tanhf, expf and the division are a few units in the last place off (2^-24 each), and 1 + erf, 1 + tanh cancel,
 so the absolute error is at most |z| 2^-21; the rounding to 16 bits adds eps / 2 of the result."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -183,6 +186,40 @@ def test_rows_apart_and_what_lies_between_them(cuda, bits, dtype, M, N, K, pad):
 
 
 @pytest.mark.parametrize("bits", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("M,N,K", [(3, 100, 64), (50, 264, 96), (300, 513, 128), (700, 1024, 72)])
+@pytest.mark.parametrize("pad,shift", [(0, 0), (8, 8), (3, 0), (7, 1), (6, 2)])
+def test_results_and_residuals_of_16_bits_anywhere(cuda, bits, dtype, M, N, K, pad, shift):
+    """Blocks of columns of wider buffers, x next to its result in one of them; what lies around them stays."""
+    x0, w, scale, _ = case(bits, M, N, K, dtype, cuda)
+    x0 = x0.clamp(-1, 1)
+    want = product(bits, x0, w, scale, out_dtype=FP32)                   # (whole numbers, exact: tested above)
+    buf = torch.full((M, K + N + pad + shift), 3.0, dtype=dtype, device=cuda)
+    x, out = buf[:, :K], buf[:, K + shift:K + shift + N]
+    x.copy_(x0)
+    res = torch.full((M, N + pad + shift), 2.0, dtype=dtype, device=cuda)
+    r = res[:, shift:shift + N]
+    product(bits, x, w, scale, residual=r, out=out)
+    assert torch.equal(out, (want + 2).to(dtype))
+    assert torch.equal(x, x0) and (buf[:, K:K + shift] == 3).all() and (buf[:, K + shift + N:] == 3).all()
+    product(bits, x, w, scale, residual=r, out=r)
+    assert torch.equal(r, (want + 2).to(dtype)) and (res[:, :shift] == 2).all() and (res[:, shift + N:] == 2).all()
+
+
+@pytest.mark.parametrize("bits", [False, True])
+def test_results_of_more_than_two_to_the_31(cuda, bits):
+    M, N, K = 66000, 33000, 40
+    x, w, scale, _ = case(bits, M, N, K, BF16, cuda)
+    out = product(bits, x, w, scale)
+    assert out.numel() > 1 << 31
+    rows = torch.tensor([0, 1, 32767, 65074, 65075, 65999], device=cuda)
+    w64 = w.double()
+    if bits:
+        w64 = torch.stack([(w[:, k // 32] >> (31 - k % 32) & 1).double() * 2 - 1 for k in range(K)], 1) * scale.double()[:, None]
+    assert torch.equal(out[rows], (x[rows].double() @ w64.t()).to(BF16))
+
+
+@pytest.mark.parametrize("bits", [False, True])
 @pytest.mark.parametrize("M,N,K", [(3, 50, 77), (500, 600, 333)])
 def test_workspaces(cuda, bits, M, N, K):
     """A workspace of one's own, for operands that need one; too small ones and none are refused by the library."""
@@ -294,6 +331,29 @@ def test_a_chain_of_dependent_calls(cuda, bits):
             want = have.double()
         else:
             assert torch.equal(have.double(), want)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: what is configured on first use is no obstacle."""
+    program = """
+import torch
+from tcbnn_b200 import ops
+x, w = torch.ones((%d, 100), dtype=torch.bfloat16, device="cuda"), torch.ones((70, 100), dtype=torch.bfloat16, device="cuda")
+bits = torch.full((70, 4), -1, dtype=torch.int32, device="cuda")
+logits = torch.ones((3, 5000), device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a, b, c = ops.linear(x, w), ops.bit_linear(x, bits), ops.log_probs(logits, None, 4)
+g.replay()
+torch.cuda.synchronize()
+assert (a == 100).all() and (b == 100).all() and c[2].tolist() == [[0, 1, 2, 3]] * 3
+print("fine")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for rows in (2, 400):
+        r = subprocess.run([sys.executable, "-c", program % rows], cwd=root, capture_output=True, text=True, timeout=300)
+        assert r.stdout.strip() == "fine", r.stderr[-2000:]
 
 
 def test_results_are_the_same_every_time(cuda):
