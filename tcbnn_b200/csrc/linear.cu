@@ -18,10 +18,10 @@ k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CU
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
     linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
 }
-template <int RT, bool BF>
-__global__ void __launch_bounds__(32 * linear::kSmallWarps, 1) k_bit_linear_small(linear::Args a) {
+template <int RT, int T, bool BF>
+__global__ void __launch_bounds__(32 * linear::small_warps(RT, T), 1) k_bit_linear_small(linear::Args a) {
     extern __shared__ __align__(16) float bit_linear_sums[];
-    linear::bit_linear_small<RT, BF>(a, bit_linear_sums);
+    linear::bit_linear_small<RT, T, BF>(a, bit_linear_sums);
 }
 template <bool BF, bool WIDE>
 __global__ void __launch_bounds__(32 * linear::kDenseWarps, 2) k_linear_small(linear::Args a) {
@@ -190,26 +190,56 @@ const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
 
 // What the launch that copies operands in front of the product takes
 double copy_time(double bytes) { return bytes > 0 ? 2.3 + bytes * 0.36e-6 : 0; }
-// Few rows: whether the kernels on warp-level MMAs are the faster ones.  Packed weights: 2.8 us and 6.5e6 expansions a us for every eight
-// rows (8192 x 8192 for 24 rows 34 us, 4096 x 4096 for 32 13, for one 4.1; the other kernel 17.5, 9.5, 8.6).  Dense ones: 2.1 us
+// How k_bit_linear_small runs: 16 x rt outputs and 8 x groups rows per block, on that many warps.
+struct SmallPlan { int rt, groups, warps; double us; };
+// The plan of least estimated time, in us at 1.9 GHz; its numbers were fitted to 822 times over 20 weights and 1 to 128 rows, and its
+// choice is 0.8 % from the best one on average (20 % at most).  A block whose SM has nothing else takes all the warps that fit, others
+// half of those, two to an SM; a warp's piece of 128 elements is paid in expansions and MMAs per 16 outputs and loads per eight rows (more of
+// them where rows start on any element), or waits for its words; then the block's sums meet.
+SmallPlan small_plan(int M, int N, int K, bool anywhere, int sms) {
+    static const int of[][2] = {{1, 1}, {1, 2}, {1, 3}, {2, 1}, {2, 2}, {2, 3}, {2, 4}, {4, 1}};
+    SmallPlan best = {0, 0, 0, 1e300};
+    const int rows = (M + 7) / 8, pieces = (K + 127) / 128;
+    for (const auto& f : of) {
+        const int rt = f[0], groups = f[1];
+        if (groups > rows) continue;
+        const int most = linear::small_warps(rt, groups);
+        const long long blocks = (long long)((N + 16 * rt - 1) / (16 * rt)) * ((rows + groups - 1) / groups);
+        const int warps = blocks <= sms ? most : 8, busy = warps < pieces ? warps : pieces, at_once = warps > 8 || most < 16 ? 1 : 2;
+        const double piece = rt * (146 + 25.0 * groups) + groups * (anywhere ? 267 : 121) + 9;
+        const double turns = (pieces + busy - 1) / busy, outputs = rt * groups * (4.0 * rt * groups > warps ? 4.0 * rt * groups / warps : 1) * busy / 16;
+        const auto wave = [&](int resident) {
+            const double clocks = resident * busy / 4.0 * piece;
+            return 1594 + turns * (clocks > 642 ? clocks : 642) + 186 * resident * outputs;
+        };
+        const long long full = blocks / (sms * at_once), rest = blocks % (sms * at_once);
+        const double us = (2357 + full * wave(at_once) + (rest ? wave(rest > sms ? 2 : 1) : 0)) / 1900;
+        if (us < best.us) best = SmallPlan{rt, groups, warps, us};
+    }
+    return best;
+}
+
+// Few rows: whether the kernels on warp-level MMAs are the faster ones, by estimates of both.  Packed weights: 1 x 4096 -> 4096 4.0 us, the
+// other kernel 8.7; 32 x 1000 -> 1000 2.6 and 7.3; 24 x 8192 -> 8192 15.6 and 17.1; 64 x 4096 -> 4096 15.0 and 11.1.  Dense ones: 2.1 us
 // and their bytes at 5.7 TB/s for every eight rows, or a warp's pieces one after another (4096 x 4096 for one row 8.3 us, 512 x 512 for 64
 // 2.4, 4096 x 9216 for 16 25; the other kernel 9.4, 4.4, 16.4); rows that start on any element at 2.6 TB/s (1 x 4097 -> 4096 15.0,
 // 32 x 1001 -> 1000 5.1, copied first 22.5, 7.8).  copied: bytes that the other kernel needs copied.
 bool small_pays(int M, int N, int K, bool bits, double copied, int sms) {
     if (M > 128 || g_linear_cols || g_linear_splits) return false;
-    const double groups = (M + 7) / 8, weights = (double)N * K;
-    double us = 2.8 + groups * weights / 6.5e6;
-    if (!bits) {
-        const double bytes = groups * 2 * weights * (copied > 0 ? 0.39e-6 : 0.175e-6), pieces = ceil(ceil(K / 128.0) / 8) * (copied > 0 ? 0.8 : 0.55);
+    double us;
+    if (bits) {
+        us = small_plan(M, N, K, copied > 0 || (K & 7), sms).us;
+    } else {
+        const double bytes = (M + 7) / 8 * 2.0 * N * K * (copied > 0 ? 0.39e-6 : 0.175e-6), pieces = ceil(ceil(K / 128.0) / 8) * (copied > 0 ? 0.8 : 0.55);
         us = 2.1 + (bytes > pieces ? bytes : pieces);
     }
     return us < plan_time(plan_linear(M, N, K, bits, sms), M, N, K, sms) + copy_time(copied);
 }
 
 // A launch of few rows' kernel: outputs x rows
-int launch_small(void (*kernel)(linear::Args), const linear::Args& a, int outputs, int threads, size_t smem, cudaStream_t st) {
+int launch_small(void (*kernel)(linear::Args), const linear::Args& a, int outputs, int rows, int threads, size_t smem, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((a.N + outputs - 1) / outputs, (a.M + 7) / 8);
+    cfg.gridDim = dim3((a.N + outputs - 1) / outputs, (a.M + rows - 1) / rows);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -264,26 +294,26 @@ int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const C
 int run_bit_linear_small(const linear::Args& a, int sms, cudaStream_t st) {
     using namespace linear;
     using Kernel = void (*)(Args);
-    static const struct { int rt; Kernel bf16, fp16; } of[] = {
-#define TCBNN_SMALL(RT) {RT, k_bit_linear_small<RT, true>, k_bit_linear_small<RT, false>}
-        TCBNN_SMALL(1), TCBNN_SMALL(2), TCBNN_SMALL(4)};
+    static const struct { int rt, groups; Kernel bf16, fp16; } of[] = {
+#define TCBNN_SMALL(RT, T) {RT, T, k_bit_linear_small<RT, T, true>, k_bit_linear_small<RT, T, false>}
+        TCBNN_SMALL(1, 1), TCBNN_SMALL(1, 2), TCBNN_SMALL(1, 3), TCBNN_SMALL(2, 1), TCBNN_SMALL(2, 2),
+        TCBNN_SMALL(2, 3), TCBNN_SMALL(2, 4), TCBNN_SMALL(4, 1)};
 #undef TCBNN_SMALL
     static bool done[64];
     if (configure_once(done, [] {
             cudaError_t e = cudaSuccess;
             for (const auto& k : of)
                 for (Kernel f : {k.bf16, k.fp16})
-                    if (e == cudaSuccess) e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small_bytes(k.rt, kSmallWarps));
+                    if (e == cudaSuccess)
+                        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)small_bytes(k.rt, k.groups, small_warps(k.rt, k.groups)));
             return e;
         })) return 1;
-    const int pieces = (a.K + 255) / 256;
-    // 16 x RT outputs per block: as many as still give every SM a block.  Sixteen warps where a block has its SM to itself: 1 x 4096 x
-    // 4096 4.1 us with RT = 2, 5.7 with 1, 6.1 with eight warps; 1 x 16384 x 4096 11.6 with RT = 4 and eight, 13.0 with sixteen.
-    const int i = a.N <= 16 * sms ? 0 : a.N <= 32 * sms ? 1 : 2, rt = of[i].rt;
-    const long long blocks = (long long)((a.N + 16 * rt - 1) / (16 * rt)) * ((a.M + 7) / 8);
-    int warps = blocks <= sms ? kSmallWarps : kSmallWarps / 2;
-    if (warps > pieces) warps = pieces;
-    return launch_small(a.type == TCBNN_BF16 ? of[i].bf16 : of[i].fp16, a, 16 * rt, 32 * warps, small_bytes(rt, warps), st);
+    const SmallPlan p = small_plan(a.M, a.N, a.K, !rows_fit(a.x, a.ldx, a.M) || (a.K & 7), sms);
+    int i = 0;
+    while (of[i].rt != p.rt || of[i].groups != p.groups) i++;
+    const int pieces = (a.K + 127) / 128;
+    return launch_small(a.type == TCBNN_BF16 ? of[i].bf16 : of[i].fp16, a, 16 * p.rt, 8 * p.groups, 32 * p.warps,
+                        small_bytes(p.rt, p.groups, pieces < p.warps ? pieces : p.warps), st);
 }
 
 int run_linear_small(const linear::Args& a, cudaStream_t st) {
@@ -291,7 +321,7 @@ int run_linear_small(const linear::Args& a, cudaStream_t st) {
     const bool wide = rows_fit(a.x, a.ldx, a.M) && rows_fit(a.W, a.ldw, a.N);
     auto kernel = a.type == TCBNN_BF16 ? wide ? k_linear_small<true, true> : k_linear_small<true, false>
                                        : wide ? k_linear_small<false, true> : k_linear_small<false, false>;
-    return launch_small(kernel, a, 16, 32 * kDenseWarps, 0, st);
+    return launch_small(kernel, a, 16, 8, 32 * kDenseWarps, 0, st);
 }
 
 int run_linear(const char* what, linear::Args a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {

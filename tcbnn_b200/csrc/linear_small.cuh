@@ -1,14 +1,16 @@
 // Products of few real-valued rows (linear.cuh) on warp-level MMAs (mma.sync m16n8k16, fp32 sums): no barrier lies in a warp's loop.  K is
 // cut into slices over a block's warps, which meet in shared memory, in order, and finish the outputs together.  The MMA's rows are
-// outputs, its columns rows of x, eight or sixteen per block; which elements of K meet in which MMA is free as long as both operands
+// outputs, its columns rows of x, eight to a tile; which elements of K meet in which MMA is free as long as both operands
 // agree, so every lane loads what lies together in memory.
 //
 // Packed weights: expanded, a weight is a sixteenth of what it weighs dense, so that with few rows neither memory nor the tensor cores
-// bound the product but the expansion, two logic operations per pair of weights, and everything that waits.  Of 256 elements lane t of the
-// four that share a row takes words 2t and 2t + 1 -- eight bytes of W, a whole sector with its neighbours -- and of x the 64 elements
-// that belong to them, 128 consecutive bytes.
+// bound the product but the expansion (a shift and a logic operation per pair of weights; three shifts of four are multiplications, on
+// the pipe that has nothing else to do), the way of x to every SM, and what waits.  One expansion serves up to 32 rows.  Lane t of the four that
+// share a row takes eight elements of every 32: 16 of 64 consecutive bytes of x, and a byte of each of the four words that all four load.  (128
+// consecutive bytes of x per lane, for whole words of W, touch four times the lines: 32 x 1000 -> 1000 5.2 us, so 2.6.)
 //
-// 1 x 4096 -> 4096 in 4.1 us, 16 x 512 -> 512 in 3.1: launch, one way from memory, expansions (1.3 us), the exchange.
+// 1 x 4096 -> 4096 in 4.0 us, 16 x 512 -> 512 in 2.0, 24 x 8192 -> 8192 in 15.6 (its MMAs 6.4): launch, one way from memory, the
+// exchange; then expansions and the loads of x, with ALUs and tensor pipe 40 % active each.
 //
 // Dense weights: memory bounds it.  A warp has 16 rows x 128 elements (4 KB) on their way while it works on the 4 KB before, 16 warps an
 // SM; lane t takes 16 bytes of every 64 of a row.  1 x 4096 -> 4096 in 8.2 us (4.1 TB/s), 1 x 4096 -> 16384 in 24.3 (5.5 TB/s, 0.85 of the
@@ -19,116 +21,18 @@
 namespace tcbnn {
 namespace linear {
 
-constexpr int kSmallWarps = 16;
-__host__ __device__ constexpr size_t small_bytes(int rt, int warps) { return (size_t)warps * 8 * (rt * 16 + 4) * 4; }
+// Most warps of a block: fewer where a warp's sums and operands need more than 128 registers
+__host__ __device__ constexpr int small_warps(int rt, int groups) { return rt * groups >= 8 ? 12 : 16; }
+__host__ __device__ constexpr size_t small_bytes(int rt, int groups, int warps) { return (size_t)warps * 8 * groups * (rt * 16 + 4) * 4; }
 
 __device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool bf16) {
     if (bf16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// eight elements of a row of x from element k on, zeros behind the last
-__device__ __forceinline__ uint4 eight(const uint16_t* row, int k, int K, bool wide) {
-    if (wide && k + 8 <= K) return ld_dep(reinterpret_cast<const uint4*>(row + k));
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-        w[i] = (k + 2 * i < K ? (uint32_t)row[k + 2 * i] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)row[k + 2 * i + 1] << 16 : 0u);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-// Sums of a block's warps, [warp][token][output] with rows of ROWS + 4, so that a warp's stores meet different banks
-template <int ROWS, int TOKENS>
-__device__ __forceinline__ void finish_small(const Args& a, const float* sums, int n0, int m0, int warps) {
-    for (int i = threadIdx.x; i < ROWS * TOKENS; i += blockDim.x) {
-        const int token = i / ROWS, o = i - token * ROWS, n = n0 + o, m = m0 + token;
-        if (m >= a.M || n >= a.N) continue;
-        float z = 0.f;
-        for (int v = 0; v < warps; v++) z += sums[(v * TOKENS + token) * (ROWS + 4) + o];
-        z = fmaf(z, a.scale ? ld_dep(a.scale + n) : 1.f, a.bias ? load(a.bias, n, a.bias_type) : 0.f);
-        z = activate(z, a.activation);
-        if (a.residual) z += load(a.residual, m * a.ldr + n, a.out_type);
-        store(a.out, m * a.ldo + n, a.out_type, z);
-    }
-}
-
-template <int RT, bool BF>
-__device__ __forceinline__ void bit_linear_small(const Args& a, float* sums) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, warps = blockDim.x >> 5;
-    const int n0 = blockIdx.x * RT * 16, m0 = blockIdx.y * 8, pieces = (a.K + 255) >> 8;
-    const bool wide = ((reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.ldx * 2)) & 15) == 0;
-    constexpr uint32_t minus = BF ? 0xBF80BF80u : 0xBC00BC00u;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    float acc[RT][4] = {};
-    const uint32_t* w_row[RT][2];
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) w_row[i][h] = reinterpret_cast<const uint32_t*>(a.W) + (long long)min(n0 + i * 16 + h * 8 + g, a.N - 1) * a.ldw + 2 * t;
-    const bool row = m0 + g < a.M;
-    const uint16_t* x_row = reinterpret_cast<const uint16_t*>(a.x) + (long long)(row ? m0 + g : 0) * a.ldx;
-    // (Behind the last word of a row there is none to load: its elements of x are zeros.)
-    auto words = [&](uint2 (&w)[RT][2], int p) {
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) w[i][h] = p * 8 + 2 * t < a.ldw ? ld_dep(reinterpret_cast<const uint2*>(w_row[i][h] + p * 8)) : make_uint2(0, 0);
-    };
-    auto elements = [&](uint4 (&x)[4], int p, int u) {   // 32 of a lane's row, those of word u
-#pragma unroll
-        for (int q = 0; q < 4; q++) x[q] = row ? eight(x_row, p * 256 + 64 * t + 32 * u + 8 * q, a.K, wide) : make_uint4(0, 0, 0, 0);
-    };
-    uint2 w[RT][2], next[RT][2];
-    uint4 x[2][4];
-    if (warp < pieces) words(w, warp);
-    for (int p = warp; p < pieces; p += warps) {
-        elements(x[0], p, 0);
-        elements(x[1], p, 1);
-        if (p + warps < pieces) words(next, p + warps);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {                    // 128 elements of K, eight MMAs
-#pragma unroll
-            for (int i = 0; i < RT; i++) {
-                // as in expand_signs, eight elements of a word at a time
-                uint32_t z[2][2];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint32_t v = u ? w[i][h].y : w[i][h].x;
-                    z[h][0] = __byte_perm(v, v << 1, 0x7632);
-                    z[h][1] = __byte_perm(v, v << 1, 0x5410);
-                }
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    uint32_t f[2][4];
-#pragma unroll
-                    for (int c = 0; c < 4; c++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) f[c >> 1][2 * (c & 1) + h] = ((z[h][q >> 1] << (2 * (4 * (q & 1) + c))) & 0x80008000u) ^ minus;
-                    mma_16(acc[i], f[0], x[u][q].x, x[u][q].y, BF);
-                    mma_16(acc[i], f[1], x[u][q].z, x[u][q].w, BF);
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int h = 0; h < 2; h++) w[i][h] = next[i][h];
-    }
-    constexpr int PITCH = RT * 16 + 4;
-#pragma unroll
-    for (int i = 0; i < RT; i++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) sums[(warp * 8 + 2 * t + (c & 1)) * PITCH + i * 16 + g + 8 * (c >> 1)] = acc[i][c];
-    __syncthreads();
-    finish_small<RT * 16, 8>(a, sums, n0, m0, warps);
-}
-
-// ---- dense weights ----------------------------------------------------------------------------------
-constexpr int kDenseWarps = 8, kDensePiece = 128;
 // Eight elements from any element on: words from the one that holds the first, turned by half a word where that is its upper half.  Words
 // behind the last element of the row are not read (`left` elements exist), elements behind it are zeros.
 __device__ __forceinline__ uint4 eight_anywhere(const uint16_t* p, int left) {
@@ -146,6 +50,107 @@ __device__ __forceinline__ uint4 eight_anywhere(const uint16_t* p, int left) {
     }
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
+
+// Sums of a block's warps, [warp][token][output] with rows of ROWS + 4, so that a warp's stores meet different banks
+template <int ROWS, int TOKENS>
+__device__ __forceinline__ void finish_small(const Args& a, const float* sums, int n0, int m0, int warps) {
+    for (int i = threadIdx.x; i < ROWS * TOKENS; i += blockDim.x) {
+        const int token = i / ROWS, o = i - token * ROWS, n = n0 + o, m = m0 + token;
+        if (m >= a.M || n >= a.N) continue;
+        float z = 0.f;
+#pragma unroll 4
+        for (int v = 0; v < warps; v++) z += sums[(v * TOKENS + token) * (ROWS + 4) + o];
+        z = fmaf(z, a.scale ? ld_dep(a.scale + n) : 1.f, a.bias ? load(a.bias, n, a.bias_type) : 0.f);
+        z = activate(z, a.activation);
+        if (a.residual) z += load(a.residual, m * a.ldr + n, a.out_type);
+        store(a.out, m * a.ldo + n, a.out_type, z);
+    }
+}
+
+template <int RT, int T, bool BF>
+__device__ __forceinline__ void bit_linear_small(const Args& a, float* sums) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, pieces = (a.K + 127) >> 7;
+    const int warps = min((int)blockDim.x >> 5, pieces), n0 = blockIdx.x * RT * 16, m0 = blockIdx.y * T * 8;
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.M > 1 ? a.ldx * 2 : 0)) & 15) == 0, eights = (a.K & 7) == 0;
+    // (factors that the compiler cannot know: one logic operation takes one constant, and a multiplication stays one)
+    const uint32_t shift[3] = {4u * blockDim.z, 16u * blockDim.z, 64u * blockDim.z}, minus = (BF ? 0xBF80BF80u : 0xBC00BC00u) * blockDim.z;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    float acc[RT][T][4] = {};
+    // (rows behind the last: the last again, whose sums nobody stores)
+    const uint32_t* w_row[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) w_row[i][h] = reinterpret_cast<const uint32_t*>(a.W) + (long long)min(n0 + i * 16 + h * 8 + g, a.N - 1) * a.ldw;
+    const uint16_t* x_row[T];
+#pragma unroll
+    for (int j = 0; j < T; j++) x_row[j] = reinterpret_cast<const uint16_t*>(a.x) + (long long)min(m0 + j * 8 + g, a.M - 1) * a.ldx + 8 * t;
+    auto words = [&](uint4 (&w)[RT][2], int p) {
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) w[i][h] = ld_dep(reinterpret_cast<const uint4*>(w_row[i][h] + p * 4));
+    };
+    auto elements = [&](uint4 (&x)[T], int p, int s) {   // eight of a lane's 32
+        const int k = p * 128 + 32 * s;
+        if (wide && (eights || p * 128 + 128 <= a.K)) {
+#pragma unroll
+            for (int j = 0; j < T; j++) x[j] = k + 8 * t < a.K ? ld_dep(reinterpret_cast<const uint4*>(x_row[j] + k)) : make_uint4(0, 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int j = 0; j < T; j++) x[j] = eight_anywhere(x_row[j] + k, a.K - k - 8 * t);
+        }
+    };
+    constexpr int AHEAD = T <= 2 ? 4 : 2;                // eights of x on their way
+    const uint32_t mine = (3 - t) << 4 | (7 - t);        // a lane's byte of two words
+    uint4 w[RT][2], x[AHEAD][T];
+    if (warp < pieces) {
+        words(w, warp);
+#pragma unroll
+        for (int s = 0; s < AHEAD; s++) elements(x[s], warp, s);
+    }
+    for (int p = warp; p < pieces; p += warps) {
+        const bool more = p + warps < pieces;
+        uint32_t v[RT][2];                               // a lane's bytes of the four words, the first on top
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) v[i][h] = __byte_perm(__byte_perm(w[i][h].z, w[i][h].w, mine), __byte_perm(w[i][h].x, w[i][h].y, mine), 0x5410);
+        if (more) words(w, p + warps);
+#pragma unroll
+        for (int s = 0; s < 4; s++) {                    // 32 elements of K, two MMAs a tile, expanded as in expand_signs
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                uint32_t f[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t z = __byte_perm(v[i][h], v[i][h] << 1, (7 - s) << 12 | (3 - s) << 4 | (7 - s) << 8 | (3 - s));
+#pragma unroll
+                    for (int c = 0; c < 4; c++) f[c >> 1][2 * (c & 1) + h] = ((c ? z * shift[c - 1] : z) & 0x80008000u) ^ minus;
+                }
+#pragma unroll
+                for (int j = 0; j < T; j++) mma_16(acc[i][j], f[0], x[s % AHEAD][j].x, x[s % AHEAD][j].y, BF);
+#pragma unroll
+                for (int j = 0; j < T; j++) mma_16(acc[i][j], f[1], x[s % AHEAD][j].z, x[s % AHEAD][j].w, BF);
+            }
+            if (s + AHEAD < 4) elements(x[s % AHEAD], p, s + AHEAD);
+            else if (more) elements(x[s % AHEAD], p + warps, s + AHEAD - 4);
+        }
+    }
+    constexpr int PITCH = RT * 16 + 4;
+#pragma unroll
+    for (int i = 0; i < RT; i++)
+#pragma unroll
+        for (int j = 0; j < T; j++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) if (warp < warps) sums[((warp * T + j) * 8 + 2 * t + (c & 1)) * PITCH + i * 16 + g + 8 * (c >> 1)] = acc[i][j][c];
+    __syncthreads();
+    finish_small<RT * 16, 8 * T>(a, sums, n0, m0, warps);
+}
+
+// ---- dense weights ----------------------------------------------------------------------------------
+constexpr int kDenseWarps = 8, kDensePiece = 128;
 // WIDE: the rows of both operands start on 16 bytes
 template <bool BF, bool WIDE>
 __device__ __forceinline__ void linear_small(const Args& a, float* sums) {

@@ -206,6 +206,21 @@ def test_results_and_residuals_of_16_bits_anywhere(cuda, bits, dtype, M, N, K, p
     assert torch.equal(r, (want + 2).to(dtype)) and (res[:, :shift] == 2).all() and (res[:, shift + N:] == 2).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 70, 100), (100, 300, 100), (60, 1000, 100), (60, 300, 1000), (33, 2000, 100), (128, 300, 1000), (24, 2000, 2049),
+                                   (16, 2100, 2049), (60, 2000, 100), (32, 2000, 1000), (33, 4000, 100), (33, 2000, 2049), (100, 1000, 333), (60, 4000, 333),
+                                   (24, 5000, 2049), (5, 5000, 1000), (24, 8192, 1001), (9, 3001, 127), (47, 600, 129), (1, 40, 100000)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("pad", [0, 3, 8])
+def test_few_rows_of_packed_weights(cuda, M, N, K, dtype, pad):
+    """Every split of few rows: 8 to 32 of them to a block, 16 to 64 outputs, warps without a piece of K, rows on 16 bytes or not."""
+    x, w, scale, sums = case(True, M, N, K, dtype, cuda)
+    wide = torch.full((M, (K + 7) // 8 * 8 + pad), math.nan, dtype=dtype, device=cuda)
+    wide[:, :K] = x
+    bias = whole(gen(M, N), (N,), 50, FP32, cuda)
+    got = ops.bit_linear(wide[:, :K], w, scale, bias, "relu", out_dtype=FP32)
+    assert torch.equal(got.double(), (sums + bias.double()).clamp(min=0))
+
+
 @pytest.mark.parametrize("bits", [False, True])
 def test_results_of_more_than_two_to_the_31(cuda, bits):
     M, N, K = 66000, 33000, 40
