@@ -1,5 +1,6 @@
 // Kernels and C ABI of the products of real-valued rows (linear.cuh) and of the scores (log_probs.cuh).
 #include "../../include/tcbnn_b200.h"
+#include <algorithm>
 #include <cmath>
 #include "host.cuh"
 #include "bnn_layers.cuh"
@@ -221,9 +222,10 @@ SmallPlan small_plan(int M, int N, int K, bool anywhere, int sms) {
 
 // Few rows: whether the kernels on warp-level MMAs are the faster ones, by estimates of both.  Packed weights: 1 x 4096 -> 4096 4.0 us, the
 // other kernel 8.7; 32 x 1000 -> 1000 2.6 and 7.3; 24 x 8192 -> 8192 15.6 and 17.1; 64 x 4096 -> 4096 15.0 and 11.1.  Dense ones: 2.1 us
-// and their bytes at 5.7 TB/s for every eight rows, or a warp's pieces one after another (4096 x 4096 for one row 8.3 us, 512 x 512 for 64
-// 2.4, 4096 x 9216 for 16 25; the other kernel 9.4, 4.4, 16.4); rows that start on any element at 2.6 TB/s (1 x 4097 -> 4096 15.0,
-// 32 x 1001 -> 1000 5.1, copied first 22.5, 7.8).  copied: bytes that the other kernel needs copied.
+// and their bytes at 5.7 TB/s for every eight rows, or a warp's pieces one after another, or 1.75 us for every wave of blocks (4096 x 4096
+// for one row 8.3 us, 512 x 512 for 64 2.4, 4096 x 9216 for 16 25, 512 -> 50000 for one 20.4; the other kernel 9.4, 4.4, 16.4, 11.8); rows
+// that start on any element at 2.6 TB/s (1 x 4097 -> 4096 15.0, 32 x 1001 -> 1000 5.1, copied first 22.5, 7.8).  copied: bytes that the
+// other kernel needs copied.
 bool small_pays(int M, int N, int K, bool bits, double copied, int sms) {
     if (M > 128 || g_linear_cols || g_linear_splits) return false;
     double us;
@@ -231,7 +233,8 @@ bool small_pays(int M, int N, int K, bool bits, double copied, int sms) {
         us = small_plan(M, N, K, copied > 0 || (K & 7), sms).us;
     } else {
         const double bytes = (M + 7) / 8 * 2.0 * N * K * (copied > 0 ? 0.39e-6 : 0.175e-6), pieces = ceil(ceil(K / 128.0) / 8) * (copied > 0 ? 0.8 : 0.55);
-        us = 2.1 + (bytes > pieces ? bytes : pieces);
+        const double blocks = (N + 15) / 16 * (double)((M + 7) / 8), waves = blocks > 2 * sms ? 1.75 * blocks / (2 * sms) : 0;
+        us = 2.1 + std::max(waves, std::max(bytes, pieces));
     }
     return us < plan_time(plan_linear(M, N, K, bits, sms), M, N, K, sms) + copy_time(copied);
 }
