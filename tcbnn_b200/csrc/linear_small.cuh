@@ -10,7 +10,7 @@
 // consecutive bytes of x per lane, for whole words of W, touch four times the lines: 32 x 1000 -> 1000 5.2 us, so 2.6.)
 //
 // 1 x 4096 -> 4096 in 4.0 us, 16 x 512 -> 512 in 2.0, 24 x 8192 -> 8192 in 15.6 (its MMAs 6.4): launch, one way from memory, the
-// exchange; then expansions and the loads of x, with ALUs and tensor pipe 40 % active each.
+// exchange; then expansions and the loads of x, with ALUs 30 % and the tensor pipe 40 % active.
 //
 // Dense weights: memory bounds it.  A warp has 16 rows x 128 elements (4 KB) on their way while it works on the 4 KB before, 16 warps an
 // SM; lane t takes 16 bytes of every 64 of a row.  1 x 4096 -> 4096 in 8.2 us (4.1 TB/s), 1 x 4096 -> 16384 in 24.3 (5.5 TB/s, 0.85 of the
