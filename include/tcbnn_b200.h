@@ -429,6 +429,10 @@ int tcbnn_linear_status(int* status);
  * of up to 128 tokens; a forced plan also keeps few rows off the kernel on warp-level MMAs.  Calls without the forced plan fail.
  * Process-wide; for tests and measurements. */
 int tcbnn_set_linear_plan(int cols, int splits);
+/* How these sizes run on a device of `sms` SMs (none is asked), rows on 16 bytes: plan[0] whether few rows' kernel on warp-level MMAs
+ * is taken; the plan of the other one: [1] its form (0 a CTA per tile, 1 K over a cluster, 2 pairs of CTAs), [2] tokens per tile, [3] CTAs
+ * that share K, [4] sets of sums, [5] columns of tensor memory, [6] stages, [7] bytes of shared memory.  For tests. */
+int tcbnn_linear_plan(int M, int N, int K, int packed, int sms, int* plan);
 /* Scores of M rows of V logits (V up to 2^30; fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
  *                                            0 for a negative target (a row without one), NaN for one past V - 1

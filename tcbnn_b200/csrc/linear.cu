@@ -167,8 +167,10 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             p.accumulators = tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192) ? 1 : 2;
             p.ring = !bits ? 0 : ((p.form == linear::SPLIT ? 256 : 512) - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
+            // (the epilogue reads 32 columns at a time of each set, the last of an odd multiple of 16 with 16 behind it)
+            const int used = p.accumulators * cols + 32 * p.ring, read = (p.accumulators - 1) * cols + ((cols + 31) & ~31);
             p.columns = 32;
-            while (p.columns < p.accumulators * cols + 32 * p.ring) p.columns *= 2;
+            while (p.columns < used || p.columns < read) p.columns *= 2;
             // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
             const size_t room = (p.form == linear::SPLIT ? 113 : 227) * 1024;
             for (p.stages = linear::kMaxStages; p.stages > 2 && linear::smem_bytes(p) > room; p.stages--) {}
@@ -419,6 +421,15 @@ int tcbnn_set_linear_plan(int cols, int splits) {
         return fail("set_linear_plan: cols is 0 or a multiple of 16 up to 256, splits is 0, 1, 2, 4 or 8, or -2 (pairs; cols a multiple of 32)");
     g_linear_cols = cols;
     g_linear_splits = splits;
+    return 0;
+}
+
+int tcbnn_linear_plan(int M, int N, int K, int packed, int sms, int* plan) {
+    if (M < 1 || N < 1 || K < 1 || M > 1 << 30 || N > 1 << 30 || K > 1 << 24 || sms < 2 || !plan) return fail("linear_plan: M, N, K >= 1, sms >= 2");
+    const linear::Plan& p = plan_linear(M, N, K, packed != 0, sms);
+    if (!p.cols) return fail("linear_plan: the forced plan does not exist for these sizes");
+    const int of[8] = {small_pays(M, N, K, packed != 0, 0, sms), p.form, p.cols, p.splits, p.accumulators, p.columns, p.stages, (int)linear::smem_bytes(p)};
+    std::copy(of, of + 8, plan);
     return 0;
 }
 
