@@ -190,6 +190,15 @@ def _rows(name, t, device, dtype, width=None, rows=None):
     raise _l.TcbnnError(f"{name}: rows must not overlap, nor the elements of a row lie apart (strides {t.stride()})")
 
 
+_MOST = (1 << 31) - 1
+
+
+def _sizes(M, N, K):
+    """Refuses what an int of the C interface does not hold (ctypes would hand on the lower 32 bits)."""
+    if M > _MOST or N > _MOST or K > _MOST:
+        raise _l.TcbnnError(f"sizes of 2^31 and more are not supported ({M}, {N}, {K})")
+
+
 def _vector(name, t, device, dtypes, n):
     """Pointer of a vector of n on the current device."""
     if t.get_device() != device or t.dtype not in dtypes or t.shape != (n,) or not t.is_contiguous():
@@ -216,6 +225,7 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
     else:
         ldw = _rows("weight", weight, device, xt, K)
         N = weight.shape[0]
+    _sizes(M, N, K)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise _l.TcbnnError(f"activation: one of {', '.join(ACTIVATIONS)} is wanted, not {activation!r}")
@@ -257,6 +267,7 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
 def linear_workspace(x, weight):
     """Scratch that linear() or bit_linear() needs on these operands, or None; without one given it is allocated per call."""
     bits = weight.dtype is torch.int32
+    _sizes(x.shape[0], weight.shape[0], x.shape[1])
     n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), None if bits else _ptr(weight), x.shape[0], weight.shape[0], x.shape[1], x.stride(0), weight.stride(0))
     return torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
 
@@ -301,6 +312,7 @@ def log_probs(logits, targets=None, top=0, temperature=1.0):
         raise _l.TcbnnError(f"logits are of torch.float32, torch.float16 or torch.bfloat16, not {logits.dtype}")
     ld = _rows("logits", logits, device, logits.dtype)
     M, V = logits.shape
+    _sizes(M, V, top)
     if not 0 <= top <= 32:
         raise _l.TcbnnError(f"top must be between 0 and 32, not {top}")
     targets_p, target_bytes = None, 0
