@@ -245,6 +245,8 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
     if workspace is not None:
         if workspace.get_device() != device:
             raise _l.TcbnnError(f"the workspace is on {workspace.device}, the current device is cuda:{device}")
+        if not workspace.is_contiguous():
+            raise _l.TcbnnError("the workspace must be contiguous")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     elif (x_p | 2 * ldx | (0 if bits else w_p | 2 * ldw)) & 15 and M:
         # (rows that do not all start on 16 bytes)

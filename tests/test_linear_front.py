@@ -46,3 +46,15 @@ def test_sizes_that_no_int_holds_are_refused(calls, call):
     with pytest.raises(lib.TcbnnError, match="2\\^31"):
         call()
     assert not calls
+
+
+@pytest.mark.parametrize("workspace", [torch.empty((1,), dtype=torch.uint8, device="meta").expand(1 << 20),
+                                       torch.empty((1 << 20, 2), dtype=torch.uint8, device="meta")[:, 0],
+                                       torch.empty((2, 1 << 20), dtype=torch.uint8, device="meta").as_strided((2, 1 << 20), (1, 1))])
+def test_workspaces_that_do_not_lie_together_are_refused(calls, workspace):
+    """Their number of elements says nothing about how much memory follows their address."""
+    with pytest.raises(lib.TcbnnError, match="contiguous"):
+        ops.linear(meta(400, 7), meta(500, 7), workspace=workspace)
+    with pytest.raises(lib.TcbnnError, match="contiguous"):
+        ops.bit_linear(meta(400, 7), meta(500, 4, dtype=torch.int32), workspace=workspace)
+    assert not calls
