@@ -410,7 +410,8 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
  * read nor written.  Sums, activation and residual are fp32, the result is rounded once.
  * residual may be out itself (same pointer and leading dimension); otherwise out shares no memory with an input.
  * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for many rows of operands that do not all start on 16 bytes
- * (they are copied to rows that do; 0 for others).  Calls that may run at the same time need workspaces of their own. */
+ * (they are copied to rows that do; 0 for others).  It shares no memory with an operand or the result, and calls that may run
+ * at the same time need workspaces of their own. */
 size_t tcbnn_linear_workspace_bytes(const void* x, const void* W, int M, int N, int K, long long ldx, long long ldw);
 int tcbnn_linear(const void* x, const void* W, const void* bias, const void* residual, void* out, int M, int N, int K, long long ldx,
                  long long ldw, long long ldr, long long ldo, int type, int out_type, int bias_type, int activation, void* workspace,

@@ -111,6 +111,21 @@ double bytes_to_copy(const void* x, const void* W, int M, int N, int K, long lon
 }
 size_t packed_bytes(int rows, int K) { return ((size_t)rows * ((K + 7) & ~7) * 2 + 255) & ~(size_t)255; }
 
+// What is copied is written while other operands are read and results stored.
+int check_workspace(const char* what, const linear::Args& a, bool bits, const void* workspace) {
+    const bool move_x = !rows_fit(a.x, a.ldx, a.M), move_w = !bits && !rows_fit(a.W, a.ldw, a.N);
+    if (!workspace || (!move_x && !move_w)) return 0;
+    const long long eb = (long long)type_bytes(a.type), ob = (long long)type_bytes(a.out_type), bb = (long long)type_bytes(a.bias_type);
+    const long long used = (long long)((move_x ? packed_bytes(a.M, a.K) : 0) + (move_w ? packed_bytes(a.N, a.K) : 0));
+    const Block room{(uintptr_t)workspace, 1, used, used};
+    const Block of[] = {{(uintptr_t)a.x, a.M, a.K * eb, a.ldx * eb}, {(uintptr_t)a.W, a.N, bits ? a.ldw * 4 : a.K * eb, bits ? a.ldw * 4 : a.ldw * eb},
+                        {(uintptr_t)a.bias, 1, a.N * bb, a.N * bb}, {(uintptr_t)a.scale, 1, 4LL * a.N, 4LL * a.N},
+                        {(uintptr_t)a.residual, a.M, a.N * ob, a.ldr * ob}, {(uintptr_t)a.out, a.M, a.N * ob, a.ldo * ob}};
+    for (const Block& b : of)
+        if (b.at && !apart(b, room)) return fail("%s: the workspace overlaps an operand or the result", what);
+    return 0;
+}
+
 int g_linear_cols = 0, g_linear_splits = 0;              // tcbnn_set_linear_plan: 0 = from the model
 
 // What a plan takes, in us at 1.9 GHz, fitted to 1400 forced plans over 22 shapes: the set-up of a launch, of a cluster's exchange, of a
@@ -332,6 +347,7 @@ int run_linear_small(const linear::Args& a, cudaStream_t st) {
 int run_linear(const char* what, linear::Args a, bool bits, void* workspace, size_t workspace_bytes, cudaStream_t st) {
     if (check_linear(what, a, bits)) return 1;
     if (a.M == 0) return 0;
+    if (check_workspace(what, a, bits, workspace)) return 1;
     int sms;
     if (sm_count(&sms)) return 1;
     const double copied = bytes_to_copy(a.x, bits ? nullptr : a.W, a.M, a.N, a.K, a.ldx, a.ldw);
