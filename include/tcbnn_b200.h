@@ -394,7 +394,7 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
 /* ---- products of real-valued rows, and scores --------------------------------------------------
  * For networks that are binary in part, e.g. heads and projections that keep 16-bit values.  No reference
  * counterparts. */
-/* Element types, and activations: z, max(z, 0), z Phi(z), its tanh form, z / (1 + e^-z). */
+/* Element types, and activations: z, max(z, 0), z Phi(z), its tanh form, z / (1 + e^-z); the last three give NaN for -inf, as -inf * 0 is. */
 #define TCBNN_FP32 0
 #define TCBNN_FP16 1
 #define TCBNN_BF16 2

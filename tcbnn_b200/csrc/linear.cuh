@@ -30,23 +30,45 @@ __device__ __forceinline__ void store(void* p, long long i, int type, float v) {
     else if (type == FP16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
     else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
-// z / (1 + e^{-z}); the exponential and the division are off by a few 2^-22 of the result, and e^{-z} by |z| 2^-23 more, which counts
-// where it is not small against 1: 2^-21 |z| in all.
-__device__ __forceinline__ float over_one_plus_exp(float z, float minus_u) { return __fdividef(z, 1.f + __expf(minus_u)); }
-// z Phi(z) by the polynomial 7.1.26 of Abramowitz and Stegun for erfc on x = |z| / sqrt 2, off by at most 1.5e-7: no cancellation for
-// negative z, and a third of the instructions of 0.5 z (1 + erff(x)).
-__device__ __forceinline__ float gelu(float z) {
-    const float x = fabsf(z) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float half = 0.5f * poly * __expf(-x * x);                     // half of erfc(x): Phi(-|z|)
-    return z * (z < 0.f ? half : 1.f - half);
+// Activations.  The accurate forms are off by a few units in the last place of the result, far out in the negative tail as well (there the
+// roundings of an exponent v weigh |v|).  The short forms are for 16-bit results of whole tiles, where their instructions show (fp32 results of
+// 1024 x 512 -> 1024 with gelu: 8.1 us, by the short form 7.4): off by about a hundredth of a rounding to 16 bits.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
+// z / (1 + e^{-v}) by the exponential of -|v|, which neither overflows nor cancels
+template <bool SHORT>
+__device__ __forceinline__ float over_one_plus_exp(float z, float v) {
+    const float w = SHORT ? __expf(-fabsf(v)) : expf(-fabsf(v));
+    return __fdividef(v < 0.f ? z * w : z, 1.f + w);
+}
+// z Phi(z), where Phi(-|z|) = e^{-z^2 / 2} Q: Q by a polynomial in t = 1 / (1 + k |z|) without constant term, the shape of 7.1.26 of Abramowitz
+// and Stegun.  Coefficients and k: least largest relative error of Q over |z| <= 13.6, behind which the product is below the normal
+// numbers; 5 units of 2^-24 as fp32 evaluates it, the short one 68.
+template <bool SHORT>
+__device__ __forceinline__ float gelu(float z) {
+    float q;
+    if (SHORT) {
+        const float t = __fdividef(1.f, fmaf(0.307591438f, fabsf(z), 1.f));
+        q = fmaf(fmaf(-0.0757672802f, t, 0.191610958f), t, 0.00538595912f);
+        q = t * fmaf(fmaf(fmaf(q, t, 0.13725508f), t, 0.118539558f), t, 0.122974204f) * ex2(-0.721347520f * z * z);
+    } else {
+        const float t = __fdividef(1.f, fmaf(0.342946798f, fabsf(z), 1.f));
+        q = fmaf(fmaf(-0.0270156274f, t, 0.140884452f), t, -0.267972608f);
+        q = fmaf(fmaf(fmaf(q, t, 0.188897667f), t, -0.0375840724f), t, 0.112119676f);
+        q = t * fmaf(fmaf(fmaf(q, t, 0.116665187f), t, 0.137205251f), t, 0.13680008f) * expf(-0.5f * (z * z));
+    }
+    return z * (z < 0.f ? q : 1.f - q);
+}
+template <bool SHORT = false>
 __device__ __forceinline__ float activate(float z, int a) {
     if (a == RELU) return z < 0.f ? 0.f : z;           // (NaN stays)
-    if (a == GELU) return gelu(z);
+    if (a == GELU) return gelu<SHORT>(z);
     // (the tanh form: 1 + tanh u = 2 / (1 + e^{-2u}))
-    if (a == GELU_TANH) return over_one_plus_exp(z, -1.59576912160573071f * (z + 0.044715f * z * z * z));
-    if (a == SILU) return over_one_plus_exp(z, -z);
+    if (a == GELU_TANH) return over_one_plus_exp<SHORT>(z, 1.59576912160573071f * (z + 0.044715f * z * z * z));
+    if (a == SILU) return over_one_plus_exp<SHORT>(z, z);
     return z;
 }
 

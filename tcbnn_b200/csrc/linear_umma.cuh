@@ -150,24 +150,24 @@ __device__ __forceinline__ float4 ld_peer4(uint32_t shared, uint32_t rank) {
     return v;
 }
 
-template <int COUNT>
+template <bool SHORT, int COUNT>
 __device__ __forceinline__ void activate_all(float (&v)[COUNT], int activation) {
     switch (activation) {
     case RELU:
 #pragma unroll
-        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], RELU);
+        for (int j = 0; j < COUNT; j++) v[j] = activate<SHORT>(v[j], RELU);
         break;
     case GELU:
 #pragma unroll
-        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU);
+        for (int j = 0; j < COUNT; j++) v[j] = activate<SHORT>(v[j], GELU);
         break;
     case GELU_TANH:
 #pragma unroll
-        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], GELU_TANH);
+        for (int j = 0; j < COUNT; j++) v[j] = activate<SHORT>(v[j], GELU_TANH);
         break;
     case SILU:
 #pragma unroll
-        for (int j = 0; j < COUNT; j++) v[j] = activate(v[j], SILU);
+        for (int j = 0; j < COUNT; j++) v[j] = activate<SHORT>(v[j], SILU);
         break;
     }
 }
@@ -186,7 +186,7 @@ struct Output {
     __device__ __forceinline__ void finish(float (&v)[COUNT], int m0, int rows) const {
 #pragma unroll
         for (int j = 0; j < COUNT; j++) v[j] = fmaf(v[j], scale, bias);
-        activate_all(v, a.activation);
+        activate_all<false>(v, a.activation);
         if (n >= a.N) return;
         if (a.residual) {
 #pragma unroll
@@ -263,7 +263,7 @@ struct Output16 {
             v[k] = fmaf(__int_as_float(lo[k]), scale[s], bias[s]);
             v[16 + k] = fmaf(__int_as_float(hi[k]), scale[2 + s], bias[2 + s]);
         }
-        activate_all(v, a.activation);
+        activate_all<true>(v, a.activation);
         const uint32_t piece = turn + (lane >> 2) * kTurnPitch + (lane & 3) * 16;       // a lane's 16 bytes
         const uint32_t row = turn + (lane & 7) * kTurnPitch + (lane >> 3) * 16;          // a fragment's row
         if (a.residual) {

@@ -62,11 +62,7 @@ constexpr float kLeastRef = -268435456.f;              // -2^28
 __host__ __device__ constexpr int list_of(int warps) { return warps < 8 ? 256 * warps : 2048; }      // keys that a row's list holds
 constexpr uint32_t kAll = 0xffffffffu;
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
+using linear::ex2;
 // order of finite values and infinities as unsigned numbers, NaN and -inf lowest
 __device__ __forceinline__ uint32_t order_of(float x) { return (uint32_t)(key_of(x, 0) >> 32); }
 
