@@ -38,11 +38,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// z / (1 + e^{-v}) by the exponential of -|v|, which neither overflows nor cancels
+// z / (1 + e^{-v}) by the exponential of -|v|, which neither overflows nor cancels; a product z e^{-|v|} below the normal numbers is 0
 template <bool SHORT>
 __device__ __forceinline__ float over_one_plus_exp(float z, float v) {
     const float w = SHORT ? __expf(-fabsf(v)) : expf(-fabsf(v));
-    return __fdividef(v < 0.f ? z * w : z, 1.f + w);
+    float y;
+    asm("div.approx.ftz.f32 %0, %1, %2;" : "=f"(y) : "f"(v < 0.f ? z * w : z), "f"(1.f + w));
+    return y;
 }
 // z Phi(z), where Phi(-|z|) = e^{-z^2 / 2} Q: Q by a polynomial in t = 1 / (1 + k |z|) without constant term, the shape of 7.1.26 of Abramowitz
 // and Stegun.  Coefficients and k: least largest relative error of Q over |z| <= 13.6, behind which the product is below the normal
