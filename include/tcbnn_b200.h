@@ -407,7 +407,9 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
  * up to 2^24).
  * x [M][ldx] and W [N][ldw] are of `type` (fp16 or bf16), bias [N] (or NULL) of that type or fp32 (bias_type), residual [M][ldr]
  * (or NULL) and out [M][ldo] of `type` or fp32 (out_type).  Leading dimensions count elements; what lies between rows is neither
- * read nor written.  Sums, activation and residual are fp32, the result is rounded once.
+ * used nor written.  Sums, activation and residual are fp32, the result is rounded once.  The tensor cores cut sums off (towards zero) at
+ * every 16 products: 4.4e-6 of a sum of 4096 on average (2-norm), 1.9e-5 of 16384, which the rounding of a 16-bit result hides; for
+ * out_type fp32 long sums are made of shorter ones, 1e-6 at any K.
  * residual may be out itself (same pointer and leading dimension); otherwise out shares no memory with an input.
  * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for many rows of operands that do not all start on 16 bytes
  * (they are copied to rows that do; 0 for others).  It shares no memory with an operand or the result, and calls that may run
@@ -432,8 +434,8 @@ int tcbnn_linear_status(int* status);
 int tcbnn_set_linear_plan(int cols, int splits);
 /* How these sizes run on a device of `sms` SMs (none is asked), rows on 16 bytes: plan[0] whether few rows' kernel on warp-level MMAs
  * is taken; the plan of the other one: [1] its form (0 a CTA per tile, 1 K over a cluster, 2 pairs of CTAs), [2] tokens per tile, [3] CTAs
- * that share K, [4] sets of sums, [5] columns of tensor memory, [6] stages, [7] bytes of shared memory.  For tests. */
-int tcbnn_linear_plan(int M, int N, int K, int packed, int sms, int* plan);
+ * that share K, [4] sets of sums, [5] columns of tensor memory, [6] stages, [7] bytes of shared memory, [8] whether sums are chained.  For tests. */
+int tcbnn_linear_plan(int M, int N, int K, int packed, int out_type, int sms, int* plan);
 /* Scores of M rows of V logits (V up to 2^30; fp32, fp16 or bf16, `ld` apart).  With d = (x - max x) / temperature and S = sum e^d over a row:
  *   logp[m]     = d(targets[m]) - ln S       targets int32 or int64 (target_bytes), or NULL (logp is not written then);
  *                                            0 for a negative target (a row without one), NaN for one past V - 1

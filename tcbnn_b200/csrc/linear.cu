@@ -13,11 +13,11 @@ namespace {
 
 __device__ int g_linear_status;      // 1 after a bounded wait inside k_linear gave up
 
-template <bool BITS, int FORM>
+template <bool BITS, int FORM, bool CHAINED>
 __global__ void __launch_bounds__(BITS ? linear::kThreadsBits : linear::kThreadsDense, FORM == linear::SPLIT ? 2 : 1)
 k_linear(linear::Args a, linear::Plan p, int* status, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x) {
     extern __shared__ __align__(128) unsigned char dyn_smem_linear[];
-    linear::umma_cta<BITS, FORM>(a, p, &map_w, &map_x, status, dyn_smem_linear);
+    linear::umma_cta<BITS, FORM, CHAINED>(a, p, &map_w, &map_x, status, dyn_smem_linear);
 }
 template <int RT, int T, bool BF>
 __global__ void __launch_bounds__(32 * linear::small_warps(RT, T), 1) k_bit_linear_small(linear::Args a) {
@@ -152,8 +152,8 @@ double plan_time(const linear::Plan& p, int M, int N, int K, int sms) {
     return (clocks / 1900 > memory ? clocks / 1900 : memory) + f.start + (pair ? f.pair : f.split[p.splits == 8 ? 3 : p.splits / 2]);
 }
 
-// The plan that takes least.
-linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
+// The plan that takes least.  exact: for fp32 results, whose sums are chained (dense weights)
+linear::Plan make_plan(int M, int N, int K, bool bits, bool exact, int sms) {
     linear::Plan best = {};
     double least = 1e300;
     const int kblocks = (K + 63) / 64, unit = bits ? 8 : 1;
@@ -175,11 +175,16 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
             const long long tiles = (long long)p.tiles_m * p.tiles_n;
             if (splits > 1 && tiles * splits > (g_linear_splits ? 1 << 20 : 3LL * sms)) continue;      // (as far as the times were fitted)
             if (g_linear_cols ? cols != g_linear_cols : cols > 32 && cols >= M + 32) continue;
+            p.chained = exact && !bits && per > linear::kChain;
+            if (p.chained && splits > 1 && cols > linear::kChainCols) {      // (no such kernel)
+                if (!g_linear_cols) continue;
+                p.chained = 0;
+            }
             p.kblocks = kblocks;
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
-            // a second set of sums where there is room, and a second tile
-            p.accumulators = tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192) ? 1 : 2;
+            // a second set of sums where there is room, and a second tile or chain
+            p.accumulators = !p.chained && (tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192)) ? 1 : 2;
             p.ring = !bits ? 0 : ((p.form == linear::SPLIT ? 256 : 512) - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
             // (the epilogue reads 32 columns at a time of each set, the last of an odd multiple of 16 with 16 behind it)
@@ -197,12 +202,12 @@ linear::Plan make_plan(int M, int N, int K, bool bits, int sms) {
 }
 
 // (The last plans of this thread: the search takes a microsecond.)
-const linear::Plan& plan_linear(int M, int N, int K, bool bits, int sms) {
-    struct Kept { int M, N, K, bits, sms, cols, splits; linear::Plan plan; };
+const linear::Plan& plan_linear(int M, int N, int K, bool bits, bool exact, int sms) {
+    struct Kept { int M, N, K, bits, exact, sms, cols, splits; linear::Plan plan; };
     static thread_local Kept kept[64];
-    Kept& k = kept[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 2246822519u ^ (unsigned)bits) >> 7 & 63];
-    if (k.M != M || k.N != N || k.K != K || k.bits != (int)bits || k.sms != sms || k.cols != g_linear_cols || k.splits != g_linear_splits)
-        k = Kept{M, N, K, (int)bits, sms, g_linear_cols, g_linear_splits, make_plan(M, N, K, bits, sms)};
+    Kept& k = kept[((unsigned)M * 2654435761u ^ (unsigned)N * 40503u ^ (unsigned)K * 2246822519u ^ (unsigned)bits * 128 ^ (unsigned)exact * 256) >> 7 & 63];
+    if (k.M != M || k.N != N || k.K != K || k.bits != (int)bits || k.exact != (int)exact || k.sms != sms || k.cols != g_linear_cols || k.splits != g_linear_splits)
+        k = Kept{M, N, K, (int)bits, (int)exact, sms, g_linear_cols, g_linear_splits, make_plan(M, N, K, bits, exact, sms)};
     return k.plan;
 }
 
@@ -253,7 +258,7 @@ bool small_pays(int M, int N, int K, bool bits, double copied, int sms) {
         const double blocks = (N + 15) / 16 * (double)((M + 7) / 8), waves = blocks > 2 * sms ? 1.75 * blocks / (2 * sms) : 0;
         us = 2.1 + std::max(waves, std::max(bytes, pieces));
     }
-    return us < plan_time(plan_linear(M, N, K, bits, sms), M, N, K, sms) + copy_time(copied);
+    return us < plan_time(plan_linear(M, N, K, bits, false, sms), M, N, K, sms) + copy_time(copied);
 }
 
 // A launch of few rows' kernel: outputs x rows
@@ -287,9 +292,11 @@ int linear_map(CUtensorMap* map, const void* base, CUtensorMapDataType type, int
 int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const CUtensorMap& map_w, const CUtensorMap& map_x, cudaStream_t st) {
     using namespace linear;
     using Kernel = void (*)(Args, Plan, int*, CUtensorMap, CUtensorMap);
-    static const struct { bool bits; int form; Kernel kernel; } of[] = {
-        {false, ALONE, k_linear<false, ALONE>}, {false, SPLIT, k_linear<false, SPLIT>}, {false, PAIR, k_linear<false, PAIR>},
-        {true, ALONE, k_linear<true, ALONE>}, {true, SPLIT, k_linear<true, SPLIT>}};
+    static const struct { bool bits; int form; bool chained; Kernel kernel; } of[] = {
+        {false, ALONE, false, k_linear<false, ALONE, false>}, {false, SPLIT, false, k_linear<false, SPLIT, false>},
+        {false, PAIR, false, k_linear<false, PAIR, false>}, {false, ALONE, true, k_linear<false, ALONE, true>},
+        {false, SPLIT, true, k_linear<false, SPLIT, true>}, {false, PAIR, true, k_linear<false, PAIR, true>},
+        {true, ALONE, false, k_linear<true, ALONE, false>}, {true, SPLIT, false, k_linear<true, SPLIT, false>}};
     static bool done[64];
     static int* status_of[64];
     int dev = 0;
@@ -301,7 +308,7 @@ int launch_linear(const linear::Args& a, const linear::Plan& p, int sms, const C
             return e != cudaSuccess ? e : cudaGetSymbolAddress((void**)&status_of[dev & 63], g_linear_status);
         })) return 1;
     int i = 0;
-    while (of[i].bits != (bool)p.bits || of[i].form != p.form) i++;
+    while (of[i].bits != (bool)p.bits || of[i].form != p.form || of[i].chained != (bool)p.chained) i++;
     const long long tiles = (long long)p.tiles_m * p.tiles_n;
     const int team = p.form == PAIR ? 2 : p.splits;
     const long long teams = p.form == SPLIT || tiles < sms / team ? tiles : sms / team;
@@ -372,7 +379,7 @@ int run_linear(const char* what, linear::Args a, bool bits, void* workspace, siz
         const cudaError_t e = launch_dependent(k_repack, (unsigned)(blocks < 16LL * sms ? blocks : 16LL * sms), 256, 0, st, moved[0], moved[1], a.K);
         if (e != cudaSuccess) return fail("%s: %s", what, cudaGetErrorString(e));
     }
-    const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, sms);
+    const linear::Plan& p = plan_linear(a.M, a.N, a.K, bits, a.out_type == TCBNN_FP32, sms);
     if (!p.cols) return fail("%s: the forced plan does not exist for these operands", what);
     const CUtensorMapDataType type = a.type == TCBNN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap map_w, map_x;
@@ -440,12 +447,12 @@ int tcbnn_set_linear_plan(int cols, int splits) {
     return 0;
 }
 
-int tcbnn_linear_plan(int M, int N, int K, int packed, int sms, int* plan) {
+int tcbnn_linear_plan(int M, int N, int K, int packed, int out_type, int sms, int* plan) {
     if (M < 1 || N < 1 || K < 1 || M > 1 << 30 || N > 1 << 30 || K > 1 << 24 || sms < 2 || !plan) return fail("linear_plan: M, N, K >= 1, sms >= 2");
-    const linear::Plan& p = plan_linear(M, N, K, packed != 0, sms);
+    const linear::Plan& p = plan_linear(M, N, K, packed != 0, out_type == TCBNN_FP32, sms);
     if (!p.cols) return fail("linear_plan: the forced plan does not exist for these sizes");
-    const int of[8] = {small_pays(M, N, K, packed != 0, 0, sms), p.form, p.cols, p.splits, p.accumulators, p.columns, p.stages, (int)linear::smem_bytes(p)};
-    std::copy(of, of + 8, plan);
+    const int of[9] = {small_pays(M, N, K, packed != 0, 0, sms), p.form, p.cols, p.splits, p.accumulators, p.columns, p.stages, (int)linear::smem_bytes(p), p.chained};
+    std::copy(of, of + 9, plan);
     return 0;
 }
 

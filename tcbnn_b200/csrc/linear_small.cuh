@@ -181,17 +181,27 @@ __device__ __forceinline__ void linear_small(const Args& a, float* sums) {
             mma_16(acc, f1, v[q][2].z, v[q][2].w, BF);
         }
     };
+    float* mine = sums + (warp * 8 + 2 * t) * 20 + g;      // a thread's four sums
+    auto add_up = [&]() {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            mine[(c & 1) * 20 + 8 * (c >> 1)] += acc[c];
+            acc[c] = 0.f;
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < 4; c++) mine[(c & 1) * 20 + 8 * (c >> 1)] = 0.f;
     uint4 v[2][4][3];
     if (warp < pieces) ask(v[0], warp);
-    for (int p = warp; p < pieces; p += 2 * kDenseWarps) {
+    for (int p = warp, turn = 0; p < pieces; p += 2 * kDenseWarps) {
+        if (turn++ == 3) { add_up(); turn = 1; }               // (chains of 768 of K: see linear_umma.cuh)
         if (p + kDenseWarps < pieces) ask(v[1], p + kDenseWarps);
         work(v[0]);
         if (p + kDenseWarps >= pieces) break;
         if (p + 2 * kDenseWarps < pieces) ask(v[0], p + 2 * kDenseWarps);
         work(v[1]);
     }
-#pragma unroll
-    for (int c = 0; c < 4; c++) sums[(warp * 8 + 2 * t + (c & 1)) * 20 + g + 8 * (c >> 1)] = acc[c];
+    add_up();
     __syncthreads();
     finish_small<16, 8>(a, sums, n0, m0, kDenseWarps);
 }

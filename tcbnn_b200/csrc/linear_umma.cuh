@@ -48,7 +48,14 @@ struct Plan {
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
     int columns;                                       // of tensor memory
+    int chained;                                       // sums in chains of kChain blocks
 };
+// The tensor cores cut an fp32 sum off at every 16 of K, always towards zero: 4.7e-7 of the result after 512 of K, 1.0e-6 after 1024, 4.4e-6
+// after 4096, 1.9e-5 after 16384 (fp32 multiply-adds: 6e-7 and 1.5e-6 at the last two).  16-bit results round that away.  For fp32
+// results of dense weights a set of sums takes chains of at most kChain blocks, and the epilogue adds the chains up in registers: 5e-7 to
+// 7e-7 at any K (fp16, whose products are longer, 6e-7 to 9.6e-7; sums that only grow 1.5e-6 and 4.3e-6).  The sets take turns as they otherwise
+// do by tiles.  4096 x 4096 -> 16384 368 -> 378 us, with gelu 391 -> 422; others as fast.  Sums of +-1 times x lose 5e-7 after 16384.
+constexpr int kChain = 12, kChainCols = 64;            // columns of a cluster's CTA, whose registers hold no more
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
 __host__ __device__ inline uint32_t stage_bytes(const Plan& p) { return (p.bits ? 0u : kWStage) + (uint32_t)own_cols(p) * 128u; }
@@ -173,6 +180,7 @@ __device__ __forceinline__ void activate_all(float (&v)[COUNT], int activation) 
 }
 // Results of fp32, and the few of a cluster's CTA: a lane has its output's scale and bias, and stores token by token, a warp 128
 // (64) consecutive bytes.
+template <bool F32>
 struct Output {
     const Args& a;
     int n;
@@ -188,14 +196,17 @@ struct Output {
         for (int j = 0; j < COUNT; j++) v[j] = fmaf(v[j], scale, bias);
         activate_all<false>(v, a.activation);
         if (n >= a.N) return;
+        const int type = F32 ? (int)FP32 : a.out_type;
         if (a.residual) {
+            long long at = m0 * a.ldr + n;
 #pragma unroll
-            for (int j = 0; j < COUNT; j++)
-                if (j < rows) v[j] += load(a.residual, (m0 + j) * a.ldr + n, a.out_type);
+            for (int j = 0; j < COUNT; j++, at += a.ldr)
+                if (j < rows) v[j] += load(a.residual, at, type);
         }
+        long long at = m0 * a.ldo + n;
 #pragma unroll
-        for (int j = 0; j < COUNT; j++)
-            if (j < rows) store(a.out, (m0 + j) * a.ldo + n, a.out_type, v[j]);
+        for (int j = 0; j < COUNT; j++, at += a.ldo)
+            if (j < rows) store(a.out, at, type, v[j]);
     }
 };
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -312,7 +323,8 @@ struct Output16 {
     }
 };
 
-template <bool BITS, int FORM>
+// CHAINED: for results of fp32
+template <bool BITS, int FORM, bool CHAINED>
 __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUtensorMap* map_w, const CUtensorMap* map_x, int* status,
                                          unsigned char* smem0) {
     using namespace umma;
@@ -384,6 +396,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const typename std::conditional<PAIRED, PairWait, WsWait>::type wait{sAbort, status};
     const uint32_t ring_col = (uint32_t)(p.accumulators * p.cols);
+    const int chains = CHAINED ? (nkb + kChain - 1) / kChain : 1, chain = CHAINED && nkb > 0 ? (nkb + chains - 1) / chains : nkb;
 
     if (warp == 8 || warp == 9) {
         // =============================== loaders ============================================
@@ -445,22 +458,25 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         bool ok = true;
         if (nkb > 0)
             for (int t = t_first; t < ntiles && ok; t += t_step) {
-                ok = wait.spin(SEMPTY(b), bph ^ 1);
-                if (!ok) break;
-                const uint32_t d = tmem + b * p.cols;
-                for (int kb = 0; kb < nkb; kb++) {
-                    if (BITS && !(ready & 2u)) ok = wait.spin(RFULL(r), rph);
-                    if (ok && !(ready & 1u)) ok = wait.spin(FULL(s), ph);
+                for (int k0 = 0; k0 < nkb && ok; k0 += chain) {          // (one turn where sums are not chained)
+                    ok = wait.spin(SEMPTY(b), bph ^ 1);
                     if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t lo = lo0 + (s * stage >> 4), x = BITS ? tmem + ring_col + r * 32 : lo;
-                    const uint32_t bar_e = EMPTY(s), bar_r = REMPTY(r), bar_c = kb + 1 == nkb ? SFULL(b) : 0u;
-                    if (++s == p.stages) { s = 0; ph ^= 1; }
-                    if (BITS && ++r == p.ring) { r = 0; rph ^= 1; }
-                    ready = mma_64<BITS, PAIRED>(leader, d, x, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > 0, FULL(s), ph, RFULL(r), rph,
-                                                 bar_e, bar_r, bar_c);
+                    const uint32_t d = tmem + b * p.cols;
+                    const int k1 = min(nkb, k0 + chain);
+                    for (int kb = k0; kb < k1; kb++) {
+                        if (BITS && !(ready & 2u)) ok = wait.spin(RFULL(r), rph);
+                        if (ok && !(ready & 1u)) ok = wait.spin(FULL(s), ph);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t lo = lo0 + (s * stage >> 4), x = BITS ? tmem + ring_col + r * 32 : lo;
+                        const uint32_t bar_e = EMPTY(s), bar_r = REMPTY(r), bar_c = kb + 1 == k1 ? SFULL(b) : 0u;
+                        if (++s == p.stages) { s = 0; ph ^= 1; }
+                        if (BITS && ++r == p.ring) { r = 0; rph ^= 1; }
+                        ready = mma_64<BITS, PAIRED>(leader, d, x, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > k0, FULL(s), ph, RFULL(r), rph,
+                                                     bar_e, bar_r, bar_c);
+                    }
+                    if (++b == p.accumulators) { b = 0; bph ^= 1; }
                 }
-                if (++b == p.accumulators) { b = 0; bph ^= 1; }
             }
         if (!ok && leader) {
             // giving up: the MMAs already issued must have finished before tensor memory is freed
@@ -527,10 +543,52 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             __syncwarp();
             if (lane == 0) { if constexpr (PAIRED) mbar_arrive_leader(SEMPTY(of)); else mbar_arrive(SEMPTY(of)); }
         };
+        auto put = [&](const auto& f, int c0, int quad) {    // sums for the cluster: [four columns][128 outputs][4]
+            float4* dst = reinterpret_cast<float4*>(smem) + (size_t)(c0 >> 2) * 128 + quad * 32 + lane;
+#pragma unroll
+            for (int j = 0; j < (int)(sizeof(f) / 16); j++)
+                if (c0 + 4 * j < p.cols) dst[j * 128] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+        };
         for (int t = t_first; t < ntiles && ok; t += t_step) {
             int tm, tn;
             tile(t, tm, tn);
             const int n0 = tn * n_of + n_own + quad * 32;
+            if constexpr (CHAINED) {
+                // a warp's pieces of 16 tokens: two of every four (32 registers at a time in place of 16: spills)
+                constexpr int PIECES = (CLUSTER ? kChainCols : kMaxCols) / 32;
+                const Output<!CLUSTER> out(a, n0 + lane);
+                const int cols = CLUSTER ? p.cols : min(p.cols, a.M - tm * p.cols);
+                auto at = [&](int i) { return half * 32 + (i >> 1) * 64 + (i & 1) * 16; };
+                float sum[PIECES][16];
+#pragma unroll
+                for (int i = 0; i < PIECES; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) sum[i][j] = 0.f;
+                for (int k0 = 0; k0 < nkb; k0 += chain) {
+                    ok = wait.relaxed(SFULL(b), bph);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++) {
+                        if (at(i) >= cols) break;
+                        int v[16];
+                        tmem_ld16(tmem + ((uint32_t)(quad * 32) << 16) + b * p.cols + at(i), v);
+                        tmem_ld_wait16(v);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sum[i][j] += __int_as_float(v[j]);
+                    }
+                    give_back(b);
+                    if (++b == p.accumulators) { b = 0; bph ^= 1; }
+                }
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    if (at(i) >= cols) break;
+                    if constexpr (CLUSTER) put(sum[i], at(i), quad);
+                    else out.finish(sum[i], tm * p.cols + at(i), min(16, cols - at(i)));
+                }
+                continue;
+            }
             const uint32_t tcol = tmem + ((uint32_t)(quad * 32) << 16) + b * p.cols;
             if (!CLUSTER && a.out_type != FP32) {
                 const Output16 out(a, smem_u32(sTurn) + warp * kTurn, n0);
@@ -555,7 +613,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                     ask(k + 1);
                 }
             } else {
-                const Output out(a, n0 + lane);
+                const Output<!CLUSTER> out(a, n0 + lane);
                 if (nkb > 0) ok = wait.relaxed(SFULL(b), bph);
                 if (!ok) break;
                 tc_fence_after();
@@ -569,11 +627,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
 #pragma unroll
                     for (int j = 0; j < 32; j++) f[j] = nkb > 0 ? __int_as_float(v[j]) : 0.f;
                     if constexpr (CLUSTER) {
-                        // sums for the cluster: [four columns][128 outputs][4]
-                        float4* dst = reinterpret_cast<float4*>(smem) + (size_t)(c0 >> 2) * 128 + quad * 32 + lane;
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (c0 + 4 * j < p.cols) dst[j * 128] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+                        put(f, c0, quad);
                     } else {
                         out.finish(f, m0, min(min(32, p.cols - c0), a.M - m0));
                     }
@@ -595,7 +649,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             const int quad = warp & 3, half = warp >> 2;
             int tm, tn;
             tile(t_first, tm, tn);
-            const Output out(a, tn * 128 + quad * 32 + lane);
+            const Output<false> out(a, tn * 128 + quad * 32 + lane);
             const int cols = min(p.cols, a.M - tm * p.cols);
             const uint32_t src = smem_u32(smem) + (uint32_t)(quad * 32 + lane) * 16u;
             for (int c = 4 * ((int)rank + half * (int)nctas); c < cols; c += 8 * (int)nctas) {

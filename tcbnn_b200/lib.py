@@ -94,7 +94,7 @@ SIGNATURES = {
     "tcbnn_linear_workspace_bytes": (_SZ, [_P, _P, _I, _I, _I, _LL, _LL]),
     "tcbnn_linear_status": (_I, [C.POINTER(C.c_int)]),
     "tcbnn_set_linear_plan": (_I, [_I, _I]),
-    "tcbnn_linear_plan": (_I, [_I, _I, _I, _I, _I, C.POINTER(C.c_int)]),
+    "tcbnn_linear_plan": (_I, [_I, _I, _I, _I, _I, _I, C.POINTER(C.c_int)]),
     "tcbnn_linear": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
     "tcbnn_bit_linear": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _LL, _LL, _LL, _LL, _I, _I, _I, _I, _P, _SZ, _P]),
     "tcbnn_set_log_probs_plan": (_I, [_I, _I]),

@@ -275,7 +275,7 @@ def linear_workspace(x, weight):
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, out=None, out_dtype=None, workspace=None):
-    """act(x @ weight.T + bias) + residual, sums in fp32, rounded once (tcbnn_linear).
+    """act(x @ weight.T + bias) + residual, sums in fp32 by the tensor cores, rounded once (tcbnn_linear; fp32 results are off by 1e-6 at any K).
     x [M][K] and weight [N][K]: bf16 or fp16, rows contiguous, any distance apart; rows that start on multiples of 16 bytes are read
     as they are, others copied first where there are many rows.  bias [N]: x's type or fp32.  residual [M][N] and out: x's type or
     fp32 (out_dtype); residual may be out itself.  activation: "none", "relu", "gelu", "gelu_tanh" or "silu".  The result carries no gradient."""

@@ -10,12 +10,12 @@ SMS = 148
 SIZES = [1, 5, 8, 16, 17, 31, 48, 64, 100, 200, 224, 256, 333, 512, 1000, 1024, 2049, 4096, 8192, 16384, 32768, 50000, 131072]
 
 
-def plan(M, N, K, packed, cols=0, splits=0):
-    """(few rows' kernel taken, form, cols, splits, sets of sums, columns of tensor memory, stages, bytes of shared memory)"""
-    of = (C.c_int * 8)()
+def plan(M, N, K, packed, cols=0, splits=0, out=lib.BF16):
+    """(few rows' kernel taken, form, cols, splits, sets of sums, columns of tensor memory, stages, bytes of shared memory, chained sums)"""
+    of = (C.c_int * 9)()
     lib.call("tcbnn_set_linear_plan", cols, splits)
     try:
-        lib.call("tcbnn_linear_plan", M, N, K, int(packed), SMS, of)
+        lib.call("tcbnn_linear_plan", M, N, K, int(packed), out, SMS, of)
     finally:
         lib.call("tcbnn_set_linear_plan", 0, 0)
     return tuple(of)
@@ -35,7 +35,7 @@ def columns_read(cols, sets):
 @pytest.mark.parametrize("packed", [False, True])
 def test_all_columns_that_are_read_are_allocated(packed):
     for M, N, K in sizes():
-        _, _, cols, _, sets, columns, _, smem = plan(M, N, K, packed)
+        _, _, cols, _, sets, columns, _, smem, _ = plan(M, N, K, packed)
         assert columns_read(cols, sets) <= columns <= 512 and columns & (columns - 1) == 0, (M, N, K, cols, sets, columns)
         assert smem <= 227 * 1024
 
@@ -46,6 +46,18 @@ def test_all_columns_of_forced_plans_are_allocated(packed, cols, splits):
     for M, N, K in [(1, 128, 64), (8, 50000, 512), (5000, 1500, 640), (4096, 16384, 4096)]:
         if splits > 1 and -(-M // cols) * -(-N // 128) * splits > 1 << 20:
             continue
-        _, _, c, _, sets, columns, _, smem = plan(M, N, K, packed, cols, splits)
+        _, _, c, _, sets, columns, _, smem, _ = plan(M, N, K, packed, cols, splits)
         assert c == cols and columns_read(c, sets) <= columns <= 512
         assert smem <= 227 * 1024
+
+
+def test_long_sums_of_fp32_results_are_chained():
+    """Dense weights: no set of sums takes more than 768 of K; two sets take turns, and a cluster's CTAs hold 64 tokens at most."""
+    for M, N, K in sizes():
+        _, form, cols, splits, sets, columns, _, smem, chained = plan(M, N, K, False, out=lib.FP32)
+        blocks = -(-(-(-K // 64)) // splits)
+        assert chained == (blocks > 12), (M, N, K, form, cols, splits)
+        if chained:
+            assert sets == 2 and (form != 1 or cols <= 64)
+        assert columns_read(cols, sets) <= columns <= (256 if form == 1 else 512) and smem <= 227 * 1024
+        assert not plan(M, N, K, False)[8] and not plan(M, N, K, True, out=lib.FP32)[8]
