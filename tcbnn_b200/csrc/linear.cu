@@ -194,6 +194,9 @@ linear::Plan make_plan(int M, int N, int K, bool bits, bool exact, int sms) {
             // A CTA of a cluster leaves room for one of the launch behind it, which is set up meanwhile.
             const size_t room = (p.form == linear::SPLIT ? 113 : 227) * 1024;
             for (p.stages = linear::kMaxStages; p.stages > 2 && linear::smem_bytes(p) > room; p.stages--) {}
+            // (two stages of 43 KB and more, or sums of 112 KB and more to exchange: 224 x 4096 -> 4096 33.5 us, with three stages 13.9; 566 x 3560
+            // -> 1504 26.9 and 24.8)
+            if (splits > 1 && p.stages < 3 && !g_linear_cols) continue;
             const double t = plan_time(p, M, N, K, sms);
             if (t < least) { least = t; best = p; }
         }

@@ -61,3 +61,13 @@ def test_long_sums_of_fp32_results_are_chained():
             assert sets == 2 and (form != 1 or cols <= 64)
         assert columns_read(cols, sets) <= columns <= (256 if form == 1 else 512) and smem <= 227 * 1024
         assert not plan(M, N, K, False)[8] and not plan(M, N, K, True, out=lib.FP32)[8]
+
+
+@pytest.mark.parametrize("out", [lib.BF16, lib.FP32])
+@pytest.mark.parametrize("packed", [False, True])
+def test_shared_sums_leave_half_an_sm_and_three_stages(packed, out):
+    """A CTA of a cluster keeps to 113 KB, two to an SM, with three stages at least."""
+    for M, N, K in sizes() + [(224, 4096, 4096), (1024, 1024, 4096), (566, 1504, 3560)]:
+        few, form, cols, _, _, _, stages, smem, _ = plan(M, N, K, packed, out=out)
+        if form == 1 and not few:
+            assert stages >= 3 and smem <= 113 * 1024, (M, N, K, cols, stages, smem)
