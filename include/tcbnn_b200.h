@@ -445,7 +445,7 @@ int tcbnn_linear_plan(int M, int N, int K, int packed, int out_type, int sms, in
  * A logit of -inf rules its token out: it has no part in the sums and is no alternative; where fewer than `top` are left the ids
  * are -1 and the log probabilities -inf.  A row with every token ruled out has entropy 0 and log probability -inf.  A row that
  * holds NaN or +inf has NaN for all of them, except that rows without a target keep 0; NaN is no alternative.
- * temperature: 1e-30 to 1e30. */
+ * temperature: 1e-30 to 1e30.  Results share no memory with the logits, the targets or one another. */
 int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, const void* targets, int target_bytes, float temperature,
                     int top, float* logp, float* entropy, int64_t* top_ids, float* top_logp, void* stream);
 

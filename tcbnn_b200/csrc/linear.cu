@@ -499,6 +499,13 @@ int tcbnn_log_probs(const void* logits, int type, int M, int V, long long ld, co
     if ((uintptr_t)logits % type_bytes(type) || (targets && (uintptr_t)targets % target_bytes) || (((uintptr_t)logp | (uintptr_t)entropy) & 3) ||
         (top && (((uintptr_t)top_ids & 7) || ((uintptr_t)top_logp & 3))))
         return fail("log_probs: a pointer is not aligned to its type");
+    const auto vector = [](const void* p, long long bytes) { return Block{(uintptr_t)p, 1, bytes, bytes}; };
+    const Block of[] = {{(uintptr_t)logits, M, V * (long long)type_bytes(type), ld * (long long)type_bytes(type)}, vector(targets, (long long)M * target_bytes),
+                        vector(targets ? logp : nullptr, 4LL * M), vector(entropy, 4LL * M), vector(top ? top_ids : nullptr, 8LL * M * top),
+                        vector(top ? top_logp : nullptr, 4LL * M * top)};
+    for (int i = 2; i < 6; i++)
+        for (int j = 0; j < i; j++)
+            if (of[i].at && of[j].at && !apart(of[j], of[i])) return fail("log_probs: results overlap the logits, the targets or one another");
     const scores::Args a{logits, targets, M, V, type, target_bytes, top, ld, 1.f / temperature, targets ? logp : nullptr, entropy,
                          (long long*)top_ids, top_logp};
     int sms;
