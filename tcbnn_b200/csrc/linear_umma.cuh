@@ -24,7 +24,7 @@
 // come from L2 and out of shared memory half as often.
 //
 // What bounds it: large products the GPU's power.  4096 x 16384 x 4096 over a second takes 400 us in pairs (1374 TFLOP/s, 1.3 GHz, 0.98 of
-// cuBLAS in the same minute), 437 without pairs, with gelu 408; packed weights 410, with gelu 456, as two sets of 256 columns do not fit
+// cuBLAS in the same minute), 437 without pairs, with gelu 417, fp32 results 436 and 493; packed weights 408, with gelu 453, as two sets of 256 columns do not fit
 // beside the expanded weights and half of an epilogue shows.  In a burst 350 (0.95 of the measured GEMM rate).  Few tokens: W's way from
 // memory, 16 x 9216 -> 4096 16.2 us for 75 MB (0.72 of the copy rate).  Between them a CTA's bytes from L2, 72 per clock, and
 // set-up and epilogue, 3 us of a launch.
