@@ -175,7 +175,9 @@ linear::Plan make_plan(int M, int N, int K, bool bits, bool exact, int sms) {
             const long long tiles = (long long)p.tiles_m * p.tiles_n;
             if (splits > 1 && tiles * splits > (g_linear_splits ? 1 << 20 : 3LL * sms)) continue;      // (as far as the times were fitted)
             if (g_linear_cols ? cols != g_linear_cols : cols > 32 && cols >= M + 32) continue;
-            p.chained = exact && !bits && per > linear::kChain;
+            const int chains = exact && !bits ? (per + linear::kChain - 1) / linear::kChain : 1;
+            const bool apart = splits > 1 && (chains - 1) * cols + ((cols + 31) & ~31) <= 256;         // (a set of sums for each)
+            p.chained = chains > 1 && !apart;
             if (p.chained && splits > 1 && cols > linear::kChainCols) {      // (no such kernel)
                 if (!g_linear_cols) continue;
                 p.chained = 0;
@@ -184,7 +186,7 @@ linear::Plan make_plan(int M, int N, int K, bool bits, bool exact, int sms) {
             p.per = per;
             p.band = cols >= 128 ? 8 : 1024 / cols;
             // a second set of sums where there is room, and a second tile or chain
-            p.accumulators = !p.chained && (tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192)) ? 1 : 2;
+            p.accumulators = apart ? chains : !p.chained && (tiles <= (pair ? sms / 2 : sms) || p.form == linear::SPLIT || (bits && cols > 192)) ? 1 : 2;
             p.ring = !bits ? 0 : ((p.form == linear::SPLIT ? 256 : 512) - p.accumulators * cols) / 32;
             if (p.ring > linear::kMaxRing) p.ring = linear::kMaxRing;
             // (the epilogue reads 32 columns at a time of each set, the last of an odd multiple of 16 with 16 behind it)

@@ -48,14 +48,14 @@ struct Plan {
     int kblocks, per;                                  // of 64; of a CTA
     int stages, ring, accumulators;                    // of x (and dense W), of expanded W, of sums
     int columns;                                       // of tensor memory
-    int chained;                                       // sums in chains of kChain blocks
+    int chained;                                       // the sets of sums take turns by chains of kChain blocks
 };
 // The tensor cores cut an fp32 sum off at every 16 of K, always towards zero: 4.7e-7 of the result after 512 of K, 1.0e-6 after 1024, 4.4e-6
 // after 4096, 1.9e-5 after 16384 (fp32 multiply-adds: 6e-7 and 1.5e-6 at the last two).  16-bit results round that away.  For fp32
 // results of dense weights a set of sums takes chains of at most kChain blocks, and the epilogue adds the chains up in registers: 5e-7 to
 // 7e-7 at any K (fp16, whose products are longer, 6e-7 to 9.6e-7; sums that only grow 1.5e-6 and 4.3e-6).  The sets take turns as they otherwise
-// do by tiles.  4096 x 4096 -> 16384 368 -> 378 us, with gelu 391 -> 422; others as fast.  Sums of +-1 times x lose 5e-7 after 16384.
-constexpr int kChain = 12, kChainCols = 64;            // columns of a cluster's CTA, whose registers hold no more
+// do by tiles, or a cluster's CTA has a set for each of its chains.  4096 x 4096 -> 16384 368 -> 378 us, with gelu 391 -> 422; smaller ones as fast on average.  Sums of +-1 times x lose 5e-7 after 16384.
+constexpr int kChain = 12, kChainCols = 64;            // columns of a cluster's CTA whose sets take turns: its registers hold no more
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
 __host__ __device__ inline uint32_t stage_bytes(const Plan& p) { return (p.bits ? 0u : kWStage) + (uint32_t)own_cols(p) * 128u; }
@@ -396,7 +396,8 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const typename std::conditional<PAIRED, PairWait, WsWait>::type wait{sAbort, status};
     const uint32_t ring_col = (uint32_t)(p.accumulators * p.cols);
-    const int chains = CHAINED ? (nkb + kChain - 1) / kChain : 1, chain = CHAINED && nkb > 0 ? (nkb + chains - 1) / chains : nkb;
+    // (one tile per cluster: its sets of sums, where there are several, are a chain each)
+    const int chains = CHAINED ? (nkb + kChain - 1) / kChain : CLUSTER ? p.accumulators : 1, chain = nkb > 0 ? (nkb + chains - 1) / chains : 0;
 
     if (warp == 8 || warp == 9) {
         // =============================== loaders ============================================
@@ -459,7 +460,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
         if (nkb > 0)
             for (int t = t_first; t < ntiles && ok; t += t_step) {
                 for (int k0 = 0; k0 < nkb && ok; k0 += chain) {          // (one turn where sums are not chained)
-                    ok = wait.spin(SEMPTY(b), bph ^ 1);
+                    if (CHAINED || !CLUSTER) ok = wait.spin(SEMPTY(b), bph ^ 1);
                     if (!ok) break;
                     const uint32_t d = tmem + b * p.cols;
                     const int k1 = min(nkb, k0 + chain);
@@ -469,7 +470,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t lo = lo0 + (s * stage >> 4), x = BITS ? tmem + ring_col + r * 32 : lo;
-                        const uint32_t bar_e = EMPTY(s), bar_r = REMPTY(r), bar_c = kb + 1 == k1 ? SFULL(b) : 0u;
+                        const uint32_t bar_e = EMPTY(s), bar_r = REMPTY(r), bar_c = kb + 1 != k1 ? 0u : CHAINED || !CLUSTER ? SFULL(b) : k1 == nkb ? SFULL(0) : 0u;
                         if (++s == p.stages) { s = 0; ph ^= 1; }
                         if (BITS && ++r == p.ring) { r = 0; rph ^= 1; }
                         ready = mma_64<BITS, PAIRED>(leader, d, x, BITS ? lo : lo + (kWStage >> 4), hi, idesc, kb > k0, FULL(s), ph, RFULL(r), rph,
@@ -627,6 +628,15 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
 #pragma unroll
                     for (int j = 0; j < 32; j++) f[j] = nkb > 0 ? __int_as_float(v[j]) : 0.f;
                     if constexpr (CLUSTER) {
+                        for (int i = 1; i * chain < nkb; i++)
+#pragma unroll
+                            for (int h = 0; h < 32; h += 16) {
+                                int more[16];
+                                tmem_ld16(tcol + i * p.cols + c0 + h, more);
+                                tmem_ld_wait16(more);
+#pragma unroll
+                                for (int j = 0; j < 16; j++) f[h + j] += __int_as_float(more[j]);
+                            }
                         put(f, c0, quad);
                     } else {
                         out.finish(f, m0, min(min(32, p.cols - c0), a.M - m0));

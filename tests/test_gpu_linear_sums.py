@@ -48,7 +48,7 @@ def test_long_sums(cuda, dtype, growing, M, N, K):
     assert off(ops.linear(x, w, out_dtype=FP32), want) <= most(dtype, growing, cuda)
 
 
-@pytest.mark.parametrize("cols,splits", [(16, 1), (48, 1), (112, 1), (128, 1), (208, 1), (256, 1), (16, 2), (48, 4), (64, 2), (64, 8), (32, -2), (96, -2), (224, -2), (256, -2)])
+@pytest.mark.parametrize("cols,splits", [(16, 1), (48, 1), (112, 1), (128, 1), (208, 1), (256, 1), (16, 2), (48, 4), (64, 2), (64, 8), (80, 2), (96, 4), (112, 8), (128, 8), (32, -2), (96, -2), (224, -2), (256, -2)])
 @pytest.mark.parametrize("M,N,K", [(1, 128, 4096), (300, 700, 1000), (530, 1300, 2000), (40, 129, 8200), (2000, 5000, 1600), (5000, 1500, 840)])
 def test_chains_of_every_plan(cuda, cols, splits, M, N, K):
     """Whole numbers: exact, whichever chain a product falls into; bias, activation and residual once."""
