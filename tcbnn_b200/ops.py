@@ -190,13 +190,11 @@ def _rows(name, t, device, dtype, width=None, rows=None):
     raise _l.TcbnnError(f"{name}: rows must not overlap, nor the elements of a row lie apart (strides {t.stride()})")
 
 
-_MOST = (1 << 31) - 1
+_MOST = (1 << 31) - 1                  # what an int of the C interface holds (ctypes would hand on the lower 32 bits of more)
 
 
-def _sizes(M, N, K):
-    """Refuses what an int of the C interface does not hold (ctypes would hand on the lower 32 bits)."""
-    if M > _MOST or N > _MOST or K > _MOST:
-        raise _l.TcbnnError(f"sizes of 2^31 and more are not supported ({M}, {N}, {K})")
+def _too_large(*sizes):
+    raise _l.TcbnnError(f"sizes of 2^31 and more are not supported {sizes}")
 
 
 def _vector(name, t, device, dtypes, n):
@@ -225,7 +223,8 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
     else:
         ldw = _rows("weight", weight, device, xt, K)
         N = weight.shape[0]
-    _sizes(M, N, K)
+    if M > _MOST or N > _MOST or K > _MOST:
+        _too_large(M, N, K)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise _l.TcbnnError(f"activation: one of {', '.join(ACTIVATIONS)} is wanted, not {activation!r}")
@@ -269,7 +268,8 @@ def _product(x, weight, scale, bias, activation, residual, out, out_dtype, works
 def linear_workspace(x, weight):
     """Scratch that linear() or bit_linear() needs on these operands, or None; without one given it is allocated per call."""
     bits = weight.dtype is torch.int32
-    _sizes(x.shape[0], weight.shape[0], x.shape[1])
+    if max(x.shape + weight.shape) > _MOST:
+        _too_large(*x.shape, *weight.shape)
     n = _l.load().tcbnn_linear_workspace_bytes(_ptr(x), None if bits else _ptr(weight), x.shape[0], weight.shape[0], x.shape[1], x.stride(0), weight.stride(0))
     return torch.empty((n,), dtype=torch.uint8, device=x.device) if n else None
 
@@ -314,7 +314,8 @@ def log_probs(logits, targets=None, top=0, temperature=1.0):
         raise _l.TcbnnError(f"logits are of torch.float32, torch.float16 or torch.bfloat16, not {logits.dtype}")
     ld = _rows("logits", logits, device, logits.dtype)
     M, V = logits.shape
-    _sizes(M, V, top)
+    if M > _MOST or V > _MOST:
+        _too_large(M, V)
     if not 0 <= top <= 32:
         raise _l.TcbnnError(f"top must be between 0 and 32, not {top}")
     targets_p, target_bytes = None, 0
