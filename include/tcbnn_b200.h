@@ -409,7 +409,7 @@ int tcbnn_bulk_copy_rate(int bytes, int depth, int warps, int ctas, int iters, d
  * (or NULL) and out [M][ldo] of `type` or fp32 (out_type).  Leading dimensions count elements; what lies between rows is neither
  * used nor written.  Sums, activation and residual are fp32, the result is rounded once.  The tensor cores cut sums off (towards zero) at
  * every 16 products: 4.4e-6 of a sum of 4096 on average (2-norm), 1.9e-5 of 16384, which the rounding of a 16-bit result hides; for
- * out_type fp32 long sums are made of shorter ones, 1e-6 at any K.
+ * out_type fp32 long sums are made of shorter ones, which leaves about 1e-6 at any K (4e-6 where all products have one sign).
  * residual may be out itself (same pointer and leading dimension); otherwise out shares no memory with an input.
  * workspace: tcbnn_linear_workspace_bytes(...) bytes, 256-byte aligned, for many rows of operands that do not all start on 16 bytes
  * (they are copied to rows that do; 0 for others).  It shares no memory with an operand or the result, and calls that may run

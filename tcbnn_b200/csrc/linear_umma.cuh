@@ -24,8 +24,8 @@
 // come from L2 and out of shared memory half as often.
 //
 // What bounds it: large products the GPU's power.  4096 x 16384 x 4096 over a second takes 400 us in pairs (1374 TFLOP/s, 1.3 GHz, 0.98 of
-// cuBLAS in the same minute), 437 without pairs, with gelu 417, fp32 results 436 and 493; packed weights 408, with gelu 453, as two sets of 256 columns do not fit
-// beside the expanded weights and half of an epilogue shows.  In a burst 350 (0.95 of the measured GEMM rate).  Few tokens: W's way from
+// cuBLAS in the same minute), 437 without pairs, with gelu 417, fp32 results 436 and 493; packed weights 408, with gelu 453, as two sets of
+// 256 columns do not fit beside the expanded weights and half of an epilogue shows.  In a burst 350 (0.95 of the measured GEMM rate).  Few tokens: W's way from
 // memory, 16 x 9216 -> 4096 16.2 us for 75 MB (0.72 of the copy rate).  Between them a CTA's bytes from L2, 72 per clock, and
 // set-up and epilogue, 3 us of a launch.
 #pragma once
@@ -53,8 +53,9 @@ struct Plan {
 // The tensor cores cut an fp32 sum off at every 16 of K, always towards zero: 4.7e-7 of the result after 512 of K, 1.0e-6 after 1024, 4.4e-6
 // after 4096, 1.9e-5 after 16384 (fp32 multiply-adds: 6e-7 and 1.5e-6 at the last two).  16-bit results round that away.  For fp32
 // results of dense weights a set of sums takes chains of at most kChain blocks, and the epilogue adds the chains up in registers: 5e-7 to
-// 7e-7 at any K (fp16, whose products are longer, 6e-7 to 9.6e-7; sums that only grow 1.5e-6 and 4.3e-6).  The sets take turns as they otherwise
-// do by tiles, or a cluster's CTA has a set for each of its chains.  4096 x 4096 -> 16384 368 -> 378 us, with gelu 391 -> 422; smaller ones as fast on average.  Sums of +-1 times x lose 5e-7 after 16384.
+// 7e-7 at any K (fp16, whose products are longer, 6e-7 to 9.6e-7; sums that only grow 1.5e-6 and 4.3e-6).  The sets take turns as they
+// otherwise do by tiles, or a cluster's CTA has a set for each of its chains.  4096 x 4096 -> 16384 368 -> 378 us, with gelu 391 -> 422;
+// smaller ones as fast on average.  Sums of +-1 times x lose 5e-7 after 16384 and are left in one chain.
 constexpr int kChain = 12, kChainCols = 64;            // columns of a cluster's CTA whose sets take turns: its registers hold no more
 // rows of x that a CTA holds of a tile
 __host__ __device__ inline int own_cols(const Plan& p) { return p.form == PAIR ? p.cols / 2 : p.cols; }
@@ -555,7 +556,7 @@ __device__ __forceinline__ void umma_cta(const Args& a, const Plan& p, const CUt
             tile(t, tm, tn);
             const int n0 = tn * n_of + n_own + quad * 32;
             if constexpr (CHAINED) {
-                // a warp's pieces of 16 tokens: two of every four (32 registers at a time in place of 16: spills)
+                // a warp's pieces of 16 tokens, two of every four (pieces of 32 spill)
                 constexpr int PIECES = (CLUSTER ? kChainCols : kMaxCols) / 32;
                 const Output<!CLUSTER> out(a, n0 + lane);
                 const int cols = CLUSTER ? p.cols : min(p.cols, a.M - tm * p.cols);
